@@ -264,6 +264,34 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
       : "memory");
 }
 
+// One lane of a converged warp (the same one every time).  A branch on it keeps
+// the MMA issue loop in uniform registers: back-to-back M = 64, N = 64 MMAs
+// measured 32 cycles apart issued this way, 45 from `if (threadIdx.x == 0)`.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
+// The weight-stationary form, kind::f16, M = 64: row r of D (N columns) lies in
+// lane r % 64 and, for the columns N/2 and up, in lane 64 + r % 64, so a result
+// takes N/2 tensor-memory columns over all 128 lanes.  N is 64, 128 or 256.
+// Measured back to back: 32 cycles at N = 64, 48 at 128, 80 at 256 (the plain
+// M = 64 form: 32, 64, 128) -- the rate of its shared-memory operands.
+__device__ __forceinline__ void mma_f16_ws_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.ws.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // Arrive (once) on `bar` when all previously issued tcgen05 async ops of this
 // thread have completed.
 __device__ __forceinline__ void mma_commit(uint64_t *bar) {

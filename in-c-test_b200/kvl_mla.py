@@ -114,6 +114,27 @@ SIGNATURES = {
     "kvl_mla_decode_step_q8": (C.c_int, [C.POINTER(KvlMlaConfig), C.POINTER(KvlMlaDeviceWeights), C.c_void_p,
                                          C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
                                          C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),
+    "kvl_mla_tree_plan_create": (C.c_int, [C.POINTER(C.c_void_p), C.c_int, i32p, i32p, i64p, C.c_int, C.c_int, C.c_int]),
+    "kvl_mla_tree_plan_destroy": (None, [C.c_void_p]),
+    "kvl_mla_tree_plan_info": (C.c_int, [C.c_void_p, i32p, i32p, i32p]),
+    "kvl_mla_tree_mask": (C.c_int, [C.POINTER(C.c_uint64), i32p, C.c_int]),
+    "kvl_mla_tree_attend_bf16": (C.c_int, [C.c_void_p] * 6 + [C.c_int64, C.c_int, C.c_int, C.c_int, C.c_float,
+                                                              C.c_void_p]),
+    "kvl_mla_tree_attend_q8": (C.c_int, [C.c_void_p] * 8 + [C.c_int64, C.c_int, C.c_int, C.c_int, C.c_float,
+                                                            C.c_void_p]),
+    "kvl_mla_tree_check": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "kvl_mla_tree_accept_bf16": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_void_p,
+                                           C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),
+    "kvl_mla_tree_accept_q8": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int,
+                                         C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p,
+                                         C.c_void_p]),
+    "kvl_mla_move_plan_create": (C.c_int, [C.POINTER(C.c_void_p), C.c_int, i64p, i64p, i64p]),
+    "kvl_mla_move_plan_destroy": (None, [C.c_void_p]),
+    "kvl_mla_move_plan_info": (C.c_int, [C.c_void_p, i32p, i64p]),
+    "kvl_mla_pool_move_bf16": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_void_p]),
+    "kvl_mla_pool_move_q8": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int,
+                                       C.c_int, C.c_void_p]),
+    "kvl_mla_move_check": (C.c_int, [C.c_void_p, C.c_void_p]),
     "kvl_mla_prefill_workspace_bytes": (C.c_size_t, [C.POINTER(KvlMlaConfig), C.c_int]),
     "kvl_mla_prefill_dev": (C.c_int, [C.POINTER(KvlMlaConfig), C.POINTER(KvlMlaDeviceWeights), C.c_void_p,
                                       C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
@@ -328,6 +349,135 @@ class AttendPlan:
         try:
             if self.h:
                 self.lib.kvl_mla_attend_plan_destroy(self.h)
+                self.h = C.c_void_p()
+        except Exception:  # noqa: BLE001 - interpreter shutdown
+            pass
+
+
+def tree_mask(parent) -> np.ndarray:
+    """kvl_mla_tree_mask: the mask words (uint64) of one tree from its nodes' parents."""
+    p = np.ascontiguousarray(parent, dtype=np.int32)
+    m = np.zeros(p.shape[0], np.uint64)
+    check(load().kvl_mla_tree_mask(ptr(m, C.POINTER(C.c_uint64)), ptr(p, i32p), p.shape[0]), "tree mask")
+    return m
+
+
+class TreePlan:
+    """kvl_mla_tree_plan_create wrapper (current CUDA device): cached lengths,
+    drafted nodes and first pool row of every sequence."""
+
+    def __init__(self, cached_len, nodes, seq_row0, num_heads=16, kv_lora_rank=512, max_ctas=0, lib=None):
+        self.lib = lib or load()
+        self.h = C.c_void_p()
+        cl = np.ascontiguousarray(cached_len, dtype=np.int32)
+        nn = np.ascontiguousarray(nodes, dtype=np.int32)
+        r0 = np.ascontiguousarray(seq_row0, dtype=np.int64)
+        if not cl.shape == nn.shape == r0.shape or cl.ndim != 1:
+            raise KvlError("tree plan: cached_len, nodes and seq_row0 have one entry per sequence")
+        self.batch, self.nodes = int(cl.shape[0]), int(nn.sum())
+        self.num_heads, self.kv_lora_rank = num_heads, kv_lora_rank
+        check(self.lib.kvl_mla_tree_plan_create(C.byref(self.h), self.batch, ptr(cl, i32p), ptr(nn, i32p),
+                                                ptr(r0, i64p), num_heads, kv_lora_rank, max_ctas), "tree plan create")
+
+    def info(self):
+        a, b, c = C.c_int(), C.c_int(), C.c_int()
+        self.lib.kvl_mla_tree_plan_info(self.h, C.byref(a), C.byref(b), C.byref(c))
+        return {"ctas": a.value, "partials": b.value, "items": c.value}
+
+    def attend_bf16(self, out, lse, q, mask, kv, rows, rope_dim=64, scale=1.0 / np.sqrt(192.0), stream=0):
+        check(self.lib.kvl_mla_tree_attend_bf16(self.h, t_ptr(out), t_ptr(lse), t_ptr(q), t_ptr(mask), t_ptr(kv),
+                                                rows, self.num_heads, self.kv_lora_rank, rope_dim, float(scale),
+                                                stream), "tree attend")
+
+    def attend_q8(self, out, lse, q, mask, lat8, lscale, rope16, rows, rope_dim=64, scale=1.0 / np.sqrt(192.0),
+                  stream=0):
+        check(self.lib.kvl_mla_tree_attend_q8(self.h, t_ptr(out), t_ptr(lse), t_ptr(q), t_ptr(mask), t_ptr(lat8),
+                                              t_ptr(lscale), t_ptr(rope16), rows, self.num_heads, self.kv_lora_rank,
+                                              rope_dim, float(scale), stream), "tree attend")
+
+    def check(self, stream=0):
+        return self.lib.kvl_mla_tree_check(self.h, stream)
+
+    def __del__(self):
+        try:
+            if self.h:
+                self.lib.kvl_mla_tree_plan_destroy(self.h)
+                self.h = C.c_void_p()
+        except Exception:  # noqa: BLE001 - interpreter shutdown
+            pass
+
+
+class PoolSet:
+    """The latent pools that one call moves rows in (1 to 64, e.g. one per
+    layer): torch tensors [pools][rows][...] or lists of [rows][...]."""
+
+    def __init__(self, arrays, widths, lib=None):
+        self.lib = lib or load()
+        self.tensors = [list(a) for a in arrays]  # keeps the pools alive
+        first = self.tensors[0]
+        self.n, self.rows = len(first), int(first[0].shape[0]) if first else 0
+        for a in self.tensors:
+            for t in a:
+                if len(a) != self.n or int(t.shape[0]) != self.rows or not t.is_contiguous():
+                    raise KvlError("pool set: contiguous arrays with the same number of pools and rows")
+        self.rank, self.rope = widths
+        self.ptrs = [(C.c_void_p * self.n)(*[t.data_ptr() for t in a]) for a in self.tensors]
+
+    @classmethod
+    def bf16(cls, kv, kv_lora_rank=512, rope_dim=64, lib=None):
+        kv = list(kv)
+        if any(t.element_size() != 2 or t.numel() != t.shape[0] * (kv_lora_rank + rope_dim) for t in kv):
+            raise KvlError("pool set: 16-bit rows of kv_lora_rank + rope_dim")
+        return cls([kv], (kv_lora_rank, rope_dim), lib)
+
+    @classmethod
+    def q8(cls, lat8, lscale, rope16, lib=None):
+        lat8, lscale, rope16 = list(lat8), list(lscale), list(rope16)
+        if not lat8 or any(t.element_size() != 1 for t in lat8) or any(t.element_size() != 4 for t in lscale) or any(
+                t.element_size() != 2 for t in rope16):
+            raise KvlError("pool set: int8 latents, fp32 row scales and 16-bit ropes")
+        rank, rope = int(lat8[0].shape[1]), int(rope16[0].shape[1])
+        if any(t.shape[1] != rank for t in lat8) or any(t.shape[1] != rope for t in rope16) or any(
+                t.numel() != t.shape[0] for t in lscale):
+            raise KvlError("pool set: pools of one row shape")
+        return cls([lat8, lscale, rope16], (rank, rope), lib)
+
+    def tree_accept(self, base, path, count, kept=None, stream=0):
+        """kvl_mla_tree_accept_*: base int64 [batch], path int32 [batch][max_path], count int32 [batch], kept int32
+        [batch] or None, on the device."""
+        fn = self.lib.kvl_mla_tree_accept_bf16 if len(self.ptrs) == 1 else self.lib.kvl_mla_tree_accept_q8
+        check(fn(*self.ptrs, self.n, self.rows, self.rank, self.rope, int(base.shape[0]), t_ptr(base), t_ptr(path),
+                 t_ptr(count), int(path.shape[1]), t_ptr(kept), stream), "tree accept")
+
+
+class PoolMovePlan:
+    """kvl_mla_move_plan_create wrapper (current CUDA device): runs of rows that are copied inside pools."""
+
+    def __init__(self, src, dst, count, lib=None):
+        self.lib = lib or load()
+        self.h = C.c_void_p()
+        s, d, n = (np.ascontiguousarray(a, dtype=np.int64) for a in (src, dst, count))
+        if not s.shape == d.shape == n.shape or s.ndim != 1:
+            raise KvlError("move plan: src, dst and count have one entry per run")
+        check(self.lib.kvl_mla_move_plan_create(C.byref(self.h), s.shape[0], ptr(s, i64p), ptr(d, i64p),
+                                                ptr(n, i64p)), "move plan create")
+
+    def info(self):
+        c, m = C.c_int(), C.c_int64()
+        self.lib.kvl_mla_move_plan_info(self.h, C.byref(c), C.byref(m))
+        return {"compaction": bool(c.value), "moved_rows": m.value}
+
+    def move(self, pools: PoolSet, stream=0):
+        fn = self.lib.kvl_mla_pool_move_bf16 if len(pools.ptrs) == 1 else self.lib.kvl_mla_pool_move_q8
+        check(fn(self.h, *pools.ptrs, pools.n, pools.rows, pools.rank, pools.rope, stream), "pool move")
+
+    def check(self, stream=0):
+        return self.lib.kvl_mla_move_check(self.h, stream)
+
+    def __del__(self):
+        try:
+            if self.h:
+                self.lib.kvl_mla_move_plan_destroy(self.h)
                 self.h = C.c_void_p()
         except Exception:  # noqa: BLE001 - interpreter shutdown
             pass

@@ -209,6 +209,101 @@ int kvl_mla_decode_step_q8(const KvlMlaConfig *cfg, const KvlMlaDeviceWeights *w
                            int64_t rows, const int64_t *d_row, const int *d_pos, int batch,
                            void *d_workspace, void *stream);
 
+/* ------------------------------------------------------------------ drafted trees */
+
+/* Speculative decoding with a tree of drafted tokens: the drafted rows are
+ * appended behind each sequence's cache, one pass attends every node of every
+ * tree, and the rows of the accepted path move up behind the cache.  (The
+ * reference verifies drafts with the linear block decode,
+ * src/mla_compressed_state.c:163-184.)
+ *
+ * Sequence b of a plan has cached_len[b] >= 0 cached rows at pool rows
+ * [seq_row0[b], seq_row0[b] + cached_len[b]) and nodes[b] (0 to 64, one at
+ * least in the batch) drafted rows right behind them; the nodes of the batch
+ * are numbered sequence by sequence.  Bit j of a node's mask word says whether
+ * it attends drafted row j of its own sequence (its own row included; bits from
+ * nodes[b] on are ignored), cached rows are attended always.  max_ctas as in
+ * kvl_mla_attend_plan_create.  A plan serves any number of calls (every layer
+ * of a step) on its device, one at a time or ordered by their streams: it owns
+ * the workspace of the split sequences.  A captured graph that holds a call
+ * must not outlive the plan, nor run at the same time as another of its calls. */
+typedef struct KvlMlaTreePlan KvlMlaTreePlan;
+
+int kvl_mla_tree_plan_create(KvlMlaTreePlan **plan, int batch, const int *cached_len, const int *nodes,
+                             const int64_t *seq_row0, int num_heads, int kv_lora_rank, int max_ctas);
+void kvl_mla_tree_plan_destroy(KvlMlaTreePlan *plan);
+/* ctas: grid size; partials: pieces of split sequences; items: all pieces. */
+int kvl_mla_tree_plan_info(const KvlMlaTreePlan *plan, int *ctas, int *partials, int *items);
+
+/* Host helper: the mask words of one tree from its nodes' parents (-1: a root;
+ * a parent comes before its children): node i attends itself and its ancestors. */
+int kvl_mla_tree_mask(uint64_t *mask, const int *parent, int nodes);
+
+/* d_q [nodes][num_heads][kv_lora_rank + rope_dim] bf16 absorbed queries, d_mask
+ * [nodes], d_out [nodes][num_heads][kv_lora_rank] bf16, d_lse [nodes]
+ * [num_heads] (natural log; may be NULL).  A node that attends no row gets 0
+ * and -inf.  What lies in rows that a node does not attend, infinities and NaN
+ * included, does not reach its result; rows behind the drafted ones are not
+ * used.  Scores, softmax sums and the accumulation are fp32; the softmax
+ * weights enter the P.V product as bf16.  The production shape (16, 512, 64)
+ * runs on the tensor cores and wants d_q, d_out and the pool's arrays 16-byte
+ * aligned; other shapes run a CUDA-core kernel.  A device-side error is
+ * reported by kvl_mla_tree_check. */
+int kvl_mla_tree_attend_bf16(const KvlMlaTreePlan *plan, uint16_t *d_out, float *d_lse, const uint16_t *d_q,
+                             const uint64_t *d_mask, const uint16_t *d_kv, int64_t rows, int num_heads,
+                             int kv_lora_rank, int rope_dim, float softmax_scale, void *stream);
+/* The same over a Q8 pool in the reference layout (as kvl_mla_attend_q8). */
+int kvl_mla_tree_attend_q8(const KvlMlaTreePlan *plan, uint16_t *d_out, float *d_lse, const uint16_t *d_q,
+                           const uint64_t *d_mask, const int8_t *d_latent_q8, const float *d_latent_scale,
+                           const uint16_t *d_rope_bf16, int64_t rows, int num_heads, int kv_lora_rank, int rope_dim,
+                           float softmax_scale, void *stream);
+/* Waits for `stream` and returns -1 if a kernel of the plan's calls reported a
+ * device-side error (a bounded wait that ran out); clears it. */
+int kvl_mla_tree_check(const KvlMlaTreePlan *plan, void *stream);
+
+/* Keeps the accepted rows of drafted trees: row d_base[b] + d_path[b][j] moves
+ * to row d_base[b] + j for j < d_count[b] (d_base[b]: the row of the tree's
+ * node 0; a path ascends, as parents come before their children), in each of
+ * n_pools pools (1 to 64, e.g. one per layer) of `rows` rows; other rows stay
+ * as they are.  d_path is [batch][max_path], max_path at most 64.  d_kept
+ * [batch] (may be NULL) receives d_count[b], or -1 where nothing was moved
+ * because the path does not ascend, leaves the pool, or shares rows with
+ * another sequence of the call.  pools: host array of device pointers. */
+int kvl_mla_tree_accept_bf16(uint16_t *const *d_pools, int n_pools, int64_t rows, int kv_lora_rank, int rope_dim,
+                             int batch, const int64_t *d_base, const int *d_path, const int *d_count, int max_path,
+                             int *d_kept, void *stream);
+int kvl_mla_tree_accept_q8(int8_t *const *d_latent_q8, float *const *d_latent_scale, uint16_t *const *d_rope_bf16,
+                           int n_pools, int64_t rows, int kv_lora_rank, int rope_dim, int batch, const int64_t *d_base,
+                           const int *d_path, const int *d_count, int max_path, int *d_kept, void *stream);
+
+/* ------------------------------------------------------------------ moving rows */
+
+/* Copies runs of rows inside pools: run i's rows [src, src + count) go to
+ * [dst, dst + count).  Two kinds: copies that read no row that is written (a
+ * sequence is forked; one source may go to several places), and compactions,
+ * whose runs all move down (dst <= src) in one order and may overlap (sequences
+ * slide together after others ended).  Every destination row receives what its
+ * source row held before the call.  Two runs that write one row, and other
+ * overlaps, are refused.  Created on and used with the current device; calls of
+ * one plan must be ordered by their streams. */
+typedef struct KvlMlaMovePlan KvlMlaMovePlan;
+
+int kvl_mla_move_plan_create(KvlMlaMovePlan **plan, int runs, const int64_t *src, const int64_t *dst,
+                             const int64_t *count);
+void kvl_mla_move_plan_destroy(KvlMlaMovePlan *plan);
+/* compaction: whether rows that are read are written too; moved_rows: rows that
+ * change their place (runs with dst == src are left out). */
+int kvl_mla_move_plan_info(const KvlMlaMovePlan *plan, int *compaction, int64_t *moved_rows);
+/* The plan's moves in each of n_pools pools (1 to 64) of `rows` rows. */
+int kvl_mla_pool_move_bf16(const KvlMlaMovePlan *plan, uint16_t *const *d_pools, int n_pools, int64_t rows,
+                           int kv_lora_rank, int rope_dim, void *stream);
+int kvl_mla_pool_move_q8(const KvlMlaMovePlan *plan, int8_t *const *d_latent_q8, float *const *d_latent_scale,
+                         uint16_t *const *d_rope_bf16, int n_pools, int64_t rows, int kv_lora_rank, int rope_dim,
+                         void *stream);
+/* Waits for `stream`; -1 if a kernel of the plan's calls reported a device-side
+ * error; clears it. */
+int kvl_mla_move_check(const KvlMlaMovePlan *plan, void *stream);
+
 /* ------------------------------------------------------------------ prefill on device */
 
 /* Scratch bytes kvl_mla_prefill_dev needs for seq_len tokens. */
