@@ -37,7 +37,6 @@ struct TreeItem {
   int nn;          // nodes of the group (1..4)
   int tile0, tile1;  // tiles [tile0, tile1)
   int slot;        // partial slot, or -1 when the chunk is the whole sequence
-  int entry;       // merge entry of the (sequence, group), or -1
 };
 
 // The (sequence, group) results that are combined from partials.

@@ -89,6 +89,41 @@ static int attend(const KvlMlaTreePlan *plan, uint16_t *out, float *lse, const u
   const bool production = nh == kHeads && R == kLatent && DR == kRope;
   if (production && ((align(out) | align(q) | align(kv) | align(lat8) | align(rope16)) & 15))
     return fail("tree attend: the queries, the output and the pool must be 16-byte aligned");
+  if (production) {
+    if (rows >= (1LL << 31)) return fail("tree attend: %lld rows", static_cast<long long>(rows));
+    TreeParams p;
+    std::memset(&p, 0, sizeof p);
+    const bool q8 = !kv;
+    const bool maps =
+        make_tmap_2d(&p.tm_q, q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kRow, (uint64_t)plan->host.nodes * kHeads, kRow * 2,
+                     64, kTreeRows, CU_TENSOR_MAP_SWIZZLE_128B) &&
+        (q8 ? make_tmap_2d(&p.tm_kv, rope16, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kRope, rows, kRope * 2, 64, kTreeKeys,
+                           CU_TENSOR_MAP_SWIZZLE_128B)
+            : make_tmap_2d(&p.tm_kv, kv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kRow, rows, kRow * 2, 64, kTreeKeys,
+                           CU_TENSOR_MAP_SWIZZLE_128B));
+    if (!maps) return fail("tree attend: tensor map");
+    p.lat8 = lat8;
+    p.lscale = lscale;
+    p.mask = mask;
+    p.out = out;
+    p.lse = lse;
+    p.part_o = static_cast<float *>(plan->d_work);
+    p.part_lse = p.part_o + (size_t)plan->host.slots * kTreeRows * kLatent;
+    p.items = reinterpret_cast<const TreeItem *>(m + plan->off_items);
+    p.cta_item = reinterpret_cast<const int *>(m + plan->off_cta);
+    p.rows = rows;
+    p.scale_log2 = scale_log2;
+    p.err = static_cast<uint32_t *>(plan->d_meta);
+    cudaError_t e = launch_tree_attend(p, q8, plan->host.grid, s);
+    if (e == cudaSuccess)
+      e = launch_tree_merge(p, reinterpret_cast<const TreeMerge *>(m + plan->off_merge),
+                            static_cast<int>(plan->host.merges.size()), plan->host.max_merge, s);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return fail("tree attend launch failed: %s", cudaGetErrorString(e));
+    }
+    return 0;
+  }
   TreeGenericParams g;
   std::memset(&g, 0, sizeof g);
   g.q = q;
