@@ -292,6 +292,25 @@ __device__ __forceinline__ void mma_f16_ws_ss(uint32_t d_tmem, uint64_t a_desc, 
       : "memory");
 }
 
+// The same with A read from tensor memory: row r, K packed two 16-bit elements a
+// column, in lane r and again in lane 64 + r (each half of the lanes multiplies
+// its own half of the N columns).  28 cycles at N = 64.
+__device__ __forceinline__ void mma_f16_ws_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.ws.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 64 rows x 16 bytes from shared memory (a matrix descriptor) into four
+// tensor-memory columns, row r to lanes r and 64 + r: the A operand above.
+__device__ __forceinline__ void tmem_cp_64x128b_x2(uint32_t taddr, uint64_t s_desc) {
+  asm volatile("tcgen05.cp.cta_group::1.64x128b.warpx2::02_13 [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
+}
+
 // Arrive (once) on `bar` when all previously issued tcgen05 async ops of this
 // thread have completed.
 __device__ __forceinline__ void mma_commit(uint64_t *bar) {

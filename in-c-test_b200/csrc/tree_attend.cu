@@ -5,7 +5,7 @@
 #include <cmath>
 #include <queue>
 
-#include "merge_core.cuh"
+#include "attend_host.cuh"
 #include "prof.cuh"
 #include "sm100.cuh"
 #include "tree_attend.cuh"
@@ -13,9 +13,10 @@
 namespace kvl {
 
 // ------------------------------------------------------------------ plan
-// What an item costs beside its tiles (query load, first tile, epilogue), a
-// partial one more (fp32 output), and the merge launch, in tiles.
-static constexpr double kItemCost = 3.0, kPartCost = 1.0, kMergeCost = 3.0;
+// In tiles (about 1.2 us): what an item costs beside its tiles (query, first
+// tile, epilogue), what the merge launch costs, and a partial's 131 KB written
+// and read.
+static constexpr double kItemCost = 3.0, kMergeCost = 3.0, kSlotCost = 0.03;
 
 int build_tree_plan(TreeHostPlan &hp, int batch, const int *cached_len, const int *nodes, const int64_t *row0,
                     int ctas) {
@@ -37,20 +38,22 @@ int build_tree_plan(TreeHostPlan &hp, int batch, const int *cached_len, const in
   }
   if (hp.nodes == 0) return -1;
 
-  // Chunk length: a sequence's tiles are cut into ceil(tiles / w) equal chunks.
-  // For a few lengths w around the share of a CTA, the items are dealt longest
-  // first to the least loaded CTA; the w whose busiest CTA ends first wins.
   struct Seq {
     int tiles, groups;
   };
   std::vector<Seq> seqs(batch);
   long long total = 0;
-  int longest = 1;
+  int longest = 1, groups = 0;
+  bool uniform = true;  // all sequences with drafted rows have as many groups
   for (int b = 0; b < batch; ++b) {
     const int keys = hp.len[b] + hp.tree[b];
     seqs[b] = {hp.tree[b] ? (keys + kTreeKeys - 1) / kTreeKeys : 0, (hp.tree[b] + kTreeGroup - 1) / kTreeGroup};
     total += (long long)seqs[b].tiles * seqs[b].groups;
     longest = std::max(longest, seqs[b].tiles);
+    if (seqs[b].groups) {
+      uniform &= groups == 0 || groups == seqs[b].groups;
+      groups = seqs[b].groups;
+    }
   }
   struct Deal {
     std::vector<TreeItem> items;
@@ -58,31 +61,78 @@ int build_tree_plan(TreeHostPlan &hp, int batch, const int *cached_len, const in
     double cost = 1e30;
   };
   Deal best;
+  auto add = [&](Deal &d, int b, int g, int tile0, int tile1, bool part) {
+    TreeItem im;
+    im.row0 = hp.row0[b];
+    im.len = hp.len[b];
+    im.tree = hp.tree[b];
+    im.node0 = hp.first_node[b] + g * kTreeGroup;
+    im.nn = std::min(kTreeGroup, hp.tree[b] - g * kTreeGroup);
+    im.tile0 = tile0;
+    im.tile1 = tile1;
+    im.slot = part ? 0 : -1;
+    d.items.push_back(im);
+  };
+  auto merge_cost = [&](int slots) { return slots ? kMergeCost + kSlotCost * slots : 0.0; };
+
+  // Equal trees: teams of `groups` CTAs, one per group, walk one concatenated
+  // list of all sequences' tiles, cut into equal ranges: no CTA has more than
+  // its share, and a range boundary splits one sequence at most.  A sequence
+  // counts kItemCost tiles more than it has; a cut within them is moved to the
+  // sequence's start.
+  const int teams = groups ? ctas / groups : 0;
+  if (uniform && teams >= 1) {
+    Deal d;
+    std::vector<double> at(batch + 1, 0.0);  // sequence starts in the list
+    for (int b = 0; b < batch; ++b) at[b + 1] = at[b] + (seqs[b].groups ? seqs[b].tiles + kItemCost : 0.0);
+    int b = 0, tile = 0, slots = 0;
+    double worst = 0;
+    for (int m = 0; m < teams; ++m) {
+      const double end = at[batch] * (m + 1) / teams;
+      double load = 0;
+      while (b < batch) {
+        if (!seqs[b].groups) {
+          ++b;
+          continue;
+        }
+        int upto = m + 1 == teams ? seqs[b].tiles : (int)std::min<double>(seqs[b].tiles, end - at[b] - kItemCost + 0.5);
+        if (seqs[b].tiles - upto <= 2 && upto > tile) upto = seqs[b].tiles;  // no crumbs
+        if (upto <= tile || (tile == 0 && upto <= 2 && upto < seqs[b].tiles)) break;
+        const bool part = tile > 0 || upto < seqs[b].tiles;
+        for (int g = 0; g < groups; ++g) {
+          add(d, b, g, tile, upto, part);
+          d.cta.push_back(m * groups + g);
+          slots += part;
+        }
+        load += upto - tile + kItemCost;
+        tile = upto;
+        if (tile < seqs[b].tiles) break;
+        ++b;
+        tile = 0;
+      }
+      worst = std::max(worst, load);
+    }
+    d.cost = worst + merge_cost(slots);
+    best = std::move(d);
+  }
+  // Otherwise a sequence's tiles are cut into ceil(tiles / w) equal chunks.  For
+  // a few lengths w around the share of a CTA, the items are dealt longest first
+  // to the least loaded CTA; the w whose busiest CTA ends first wins.
   const double share = (double)total / ctas;
-  for (double f : {1e9, 1.0, 0.5, 0.34, 0.25, 0.125}) {
+  for (double f : {1e9, 1.0, 0.5, 0.34, 0.25, 0.17}) {
     const int w = (int)std::min<double>(longest, std::max(1.0, std::ceil(f * share)));
     Deal d;
-    int slots = 0, most = 0;
+    int slots = 0;
     for (int b = 0; b < batch; ++b) {
       if (!seqs[b].groups) continue;
       const int n = (seqs[b].tiles + w - 1) / w;
-      most = std::max(most, n);
       for (int c = 0; c < n; ++c)
         for (int g = 0; g < seqs[b].groups; ++g) {
-          TreeItem im;
-          im.row0 = hp.row0[b];
-          im.len = hp.len[b];
-          im.tree = hp.tree[b];
-          im.node0 = hp.first_node[b] + g * kTreeGroup;
-          im.nn = std::min(kTreeGroup, hp.tree[b] - g * kTreeGroup);
-          im.tile0 = (int)((long long)seqs[b].tiles * c / n);
-          im.tile1 = (int)((long long)seqs[b].tiles * (c + 1) / n);
-          im.slot = n > 1 ? 0 : -1;
+          add(d, b, g, (int)((long long)seqs[b].tiles * c / n), (int)((long long)seqs[b].tiles * (c + 1) / n), n > 1);
           slots += n > 1;
-          d.items.push_back(im);
         }
     }
-    if (d.items.size() > 65536 && best.cost < 1e30) continue;
+    if (d.items.size() > 16384 && best.cost < 1e30) continue;
     std::vector<int> order(d.items.size());
     for (size_t i = 0; i < order.size(); ++i) order[i] = (int)i;
     auto size = [&](int i) { return d.items[i].tile1 - d.items[i].tile0; };
@@ -95,12 +145,12 @@ int build_tree_plan(TreeHostPlan &hp, int batch, const int *cached_len, const in
     for (int i : order) {
       Load l = heap.top();
       heap.pop();
-      l.first += size(i) + kItemCost + (d.items[i].slot >= 0 ? kPartCost : 0.0);
+      l.first += size(i) + kItemCost;
       end = std::max(end, l.first);
       d.cta[i] = l.second;
       heap.push(l);
     }
-    d.cost = end + (most > 1 ? kMergeCost + 0.02 * most + 0.01 * slots : 0.0);
+    d.cost = end + merge_cost(slots);
     if (d.cost < best.cost) best = std::move(d);
   }
   // items of a CTA in the order of the plan; empty CTAs are left out
@@ -240,39 +290,48 @@ cudaError_t launch_tree_generic(const TreeGenericParams &p, int nodes, cudaStrea
 namespace treek {
 
 constexpr uint32_t kBox = kTreeKeys * 128;  // 64 rows x 64 dims bf16 = 8 KB, one SW128 box
-constexpr int kBoxes = kRow / 64;           // 8 latent boxes and the rope box
-constexpr int kStages = 2;                  // key tiles in shared memory
-constexpr uint32_t kStage = kBoxes * kBox;
-constexpr uint32_t OFF_Q = 0;
-constexpr uint32_t OFF_KV = OFF_Q + kBoxes * kBox;
-constexpr uint32_t OFF_P = OFF_KV + kStages * kStage;
-constexpr uint32_t OFF_BAR = OFF_P + kBox;
+constexpr uint32_t kUnit = 4 * kBox;        // half a tile's latents: 64 rows x 256 dims
 
-// The three pieces of a tile in the order they are loaded: rope, latent dims
-// 0-255, latent dims 256-511.  The rope is free once the scores are done, each
-// latent half once its half of the P.V is.
-enum { CH_ROPE = 0, CH_LO = 1, CH_HI = 2, kChunks = 3 };
+// Shared memory and tensor memory.  The score MMA reads its query rows from
+// tensor memory as far as they fit there (kQT boxes of 64 dims), so that shared
+// memory holds three key tiles: while the scores of tile g + 1 run, tile g
+// waits for its P.V and tile g + 2 is on its way.  With the whole query in
+// shared memory and two tiles (scores and P.V of a tile in turn) a tile took
+// 3420 cycles, of which the tensor core worked about 1750.
+//   bf16: scores 32 columns, 7 query boxes in tensor memory, 2 in shared memory
+//   Q8:   scores 64 columns (the latents' part takes the row scale afterwards,
+//         the rope's does not), 6 and 3; two and a half tiles, the converter
+//         warps hold the next one in registers
+template <bool Q8>
+struct Cfg {
+  static constexpr int kUnits = Q8 ? 5 : 6;
+  static constexpr int kQT = Q8 ? 6 : 7, kQS = 9 - kQT;
+  static constexpr uint32_t OFF_RP = kUnits * kUnit;         // rope of a tile, then its P: two boxes
+  static constexpr uint32_t OFF_QS = OFF_RP + 2 * kBox;
+  static constexpr uint32_t OFF_BAR = OFF_QS + kQS * kBox;
+  // O (64 rows x 512) takes 256 columns: dims [256 i, 256 i + 128) in columns
+  // [128 i, 128 i + 128) of lanes 0-63, the next 128 dims in lanes 64-127.
+  static constexpr uint32_t kColS = 256, kColQ = kColS + (Q8 ? 64 : 32);
+  static_assert(kColQ + 32 * kQT == 512, "tensor memory");
+};
+constexpr uint32_t kTmemCols = 512;
+constexpr int kScaleRing = 4;
 
 struct Bars {
-  uint64_t full[kStages][kChunks], empty[kStages][kChunks];
-  uint64_t q_full, q_empty;
-  uint64_t s_full[2], s_empty[2];
+  uint64_t lat_full[6], lat_empty[6];
+  uint64_t rp_full[2], rp_empty[2];  // empty: the tile's P.V is done
+  uint64_t qs_full, q_done;          // q_done: the item's last scores are done
+  uint64_t s_full, s_empty;
   uint64_t p_full, pv_done, o_empty, drain;
   uint32_t tmem_base;
   int abort;
   uint32_t nonfinite[4];
   float red[3][128];  // row maxima of alternate tiles; row sums at an item's end
-  float scale[kStages][kTreeKeys];  // Q8: row scales of the tile
+  float scale[kScaleRing][kTreeKeys];  // Q8: row scales of the tiles in flight
 };
-constexpr uint32_t kSmemBytes = OFF_BAR + sizeof(Bars);
-static_assert(kSmemBytes <= 232448, "shared memory budget");
-
-// Tensor memory: O (64 rows x 512) in 256 columns -- dims [256 i, 256 i + 128)
-// in columns [128 i, 128 i + 128) of lanes 0-63, the next 128 dims in lanes
-// 64-127 -- and two score buffers of 64 columns (32 latent; Q8: 32 more rope).
-constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kColS = 256;
-constexpr uint32_t kSCols = 64;
+template <bool Q8>
+constexpr uint32_t smem_bytes() { return Cfg<Q8>::OFF_BAR + sizeof(Bars); }
+static_assert(smem_bytes<false>() <= 232448 && smem_bytes<true>() <= 232448, "shared memory budget");
 
 constexpr int kConvertWarp = 8;  // Q8: warps 8-15 load and convert the latents
 constexpr int kConvertThreads = 256;
@@ -283,6 +342,16 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Matrix descriptor of a SW128 operand from its low word; the high word (8-row
+// groups 1024 bytes apart) is the same for all of them.
+__device__ __forceinline__ uint64_t desc_of(uint32_t lo) {
+  constexpr uint32_t hi = (1024 >> 4) | (1u << 14) | (LAYOUT_SW128 << 29);
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo_bytes) {
+  return saddr >> 4 | (lbo_bytes >> 4) << 16;
 }
 
 // Two of the four int8 in `w` (bytes i, i + 1) as bf16.  0x4300 is 128 with a
@@ -302,16 +371,21 @@ __device__ __forceinline__ uint32_t s8x2_to_bf16(uint32_t w) {
 using namespace treek;
 
 // One CTA per SM, roles by warp:
-//   0      TMA producer (bf16: whole rows; Q8: the rope)
+//   0      TMA producer: queries, ropes, bf16 latents
 //   1      tcgen05 issuer
-//   2      query loader: 64 rows x 576 per item
+//   2      loader of the query boxes that stay in shared memory
 //   4-7    softmax and epilogue: thread t has query row t % 64 and keys
 //          32 (t / 64) .. + 31 of a tile (where .ws puts them)
 //   8-15   Q8: latents from global memory, as bf16 into the ring
+//
+// The latent ring runs in units of half a tile.  An item starts with two units
+// of query boxes, which the issuer copies to tensor memory (tcgen05.cp).  A
+// tile's rope box is read by the scores only; its P then takes the same place.
 template <bool Q8>
 __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __grid_constant__ TreeParams p) {
+  using C = Cfg<Q8>;
   extern __shared__ __align__(1024) uint8_t smem[];
-  Bars *B = reinterpret_cast<Bars *>(smem + OFF_BAR);
+  Bars *B = reinterpret_cast<Bars *>(smem + C::OFF_BAR);
   const uint32_t s_base = smem_u32(smem);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -319,17 +393,18 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
   volatile int *abort = &B->abort;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i)
-      for (int c = 0; c < kChunks; ++c) {
-        mbar_init(&B->full[i][c], Q8 && c != CH_ROPE ? kConvertThreads / 32 : 1);
-        mbar_init(&B->empty[i][c], 1);
-      }
-    mbar_init(&B->q_full, 1);
-    mbar_init(&B->q_empty, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&B->s_full[i], 1);
-      mbar_init(&B->s_empty[i], 4);
+    for (int i = 0; i < 6; ++i) {
+      mbar_init(&B->lat_full[i], Q8 ? kConvertThreads / 32 : 1);
+      mbar_init(&B->lat_empty[i], 1);
     }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&B->rp_full[i], 1);
+      mbar_init(&B->rp_empty[i], 1);
+    }
+    mbar_init(&B->qs_full, 1);
+    mbar_init(&B->q_done, 1);
+    mbar_init(&B->s_full, 1);
+    mbar_init(&B->s_empty, 4);
     mbar_init(&B->p_full, 4);
     mbar_init(&B->pv_done, 1);
     mbar_init(&B->o_empty, 4);
@@ -352,262 +427,333 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
   const bool fit = !*abort;  // the same for all threads
   asm volatile("griddepcontrol.launch_dependents;");
 
-  if (warp == 0 && fit) {
-    if (elect_one()) {
-      tma_prefetch_desc(&p.tm_kv);
-      uint32_t g = 0, issued = 0;  // chunks issued
-      bool ok = true;
-      for (int it = it0; it < it1 && ok; ++it) {
-        const TreeItem im = p.items[it];
-        for (int t = im.tile0; t < im.tile1 && ok; ++t, ++g) {
-          const uint32_t st = g % kStages, par = ((g / kStages) & 1) ^ 1;
-          const int32_t y = static_cast<int32_t>(im.row0 + static_cast<long long>(kTreeKeys) * t);
-          uint8_t *dst = smem + OFF_KV + st * kStage;
-          for (int c = 0; c < (Q8 ? 1 : kChunks); ++c) {
-            ok = mbar_wait(&B->empty[st][c], par, abort, p.err, ERR_TIMEOUT_EMPTY);
+  // Q8: 512 threads start with 128 registers each; 96 + 160 + 2 x 128 = 4 x 128
+  if (warp < 4) {
+    if (Q8) asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    if (warp == 0 && fit) {
+      if (elect_one()) {
+        tma_prefetch_desc(&p.tm_q);
+        tma_prefetch_desc(&p.tm_kv);
+        uint32_t g = 0, u = 0, rp = 0;  // u: units of the ring so far, rp: ropes issued
+        bool ok = true;
+        for (int it = it0; it < it1 && ok; ++it) {
+          const TreeItem im = p.items[it];
+          for (int h = 0; h < 2 && ok; ++h, ++u) {
+            const uint32_t s = u % C::kUnits;
+            ok = mbar_wait(&B->lat_empty[s], ((u / C::kUnits) & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY);
             if (!ok) break;
-            if (c == CH_ROPE) {
-              mbar_arrive_expect_tx(&B->full[st][c], kBox);
-              tma_load_2d(dst + 8 * kBox, &p.tm_kv, &B->full[st][c], Q8 ? 0 : kLatent, y);
-            } else {
-              mbar_arrive_expect_tx(&B->full[st][c], 4 * kBox);
-              for (int b = 4 * (c - 1); b < 4 * c; ++b)
-                tma_load_2d(dst + b * kBox, &p.tm_kv, &B->full[st][c], 64 * b, y);
+            const int n = h ? C::kQT - 4 : 4;
+            mbar_arrive_expect_tx(&B->lat_full[s], n * kBox);
+            for (int b = 0; b < n; ++b)
+              tma_load_2d(smem + s * kUnit + b * kBox, &p.tm_q, &B->lat_full[s], 64 * (4 * h + b), im.node0 * kHeads);
+            if (Q8)  // the barrier counts the converter warps
+              for (int i = 1; i < kConvertThreads / 32; ++i) mbar_arrive(&B->lat_full[s]);
+          }
+          for (int t = im.tile0; t < im.tile1 && ok; ++t, ++g) {
+            const int32_t y = static_cast<int32_t>(im.row0 + static_cast<long long>(kTreeKeys) * t);
+            for (int h = 0; h < 2 && ok; ++h, ++u) {
+              if (Q8) continue;
+              const uint32_t s = u % C::kUnits;
+              ok = mbar_wait(&B->lat_empty[s], ((u / C::kUnits) & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY);
+              if (!ok) break;
+              mbar_arrive_expect_tx(&B->lat_full[s], kUnit);
+              for (int b = 0; b < 4; ++b)
+                tma_load_2d(smem + s * kUnit + b * kBox, &p.tm_kv, &B->lat_full[s], 64 * (4 * h + b), y);
             }
-            ++issued;
+            if (!ok) break;
+            ok = mbar_wait(&B->rp_empty[g & 1], ((g >> 1) & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY);
+            if (!ok) break;
+            mbar_arrive_expect_tx(&B->rp_full[g & 1], kBox);
+            tma_load_2d(smem + C::OFF_RP + (g & 1) * kBox, &p.tm_kv, &B->rp_full[g & 1], Q8 ? 0 : kLatent, y);
+            rp = g + 1;
+          }
+        }
+        if (!ok) {  // copies in flight land before the CTA exits
+          for (uint32_t k = u > C::kUnits ? u - C::kUnits : 0; !Q8 && k < u; ++k)
+            drain_wait(&B->lat_full[k % C::kUnits], (k / C::kUnits) & 1, p.err);
+          for (uint32_t k = rp > 2 ? rp - 2 : 0; k < rp; ++k) drain_wait(&B->rp_full[k & 1], (k >> 1) & 1, p.err);
+          if (Q8) {  // query units: no barrier phase is left to wait on for sure, so wait long enough
+            const uint64_t t0 = globaltimer();
+            while (globaltimer() - t0 < 1000000ull) {
+            }
           }
         }
       }
-      if (!ok) {  // copies in flight land before the CTA exits
-        const uint32_t per = Q8 ? 1 : kChunks;
-        for (uint32_t k = issued > kStages * per ? issued - kStages * per : 0; k < issued; ++k)
-          drain_wait(&B->full[(k / per) % kStages][k % per], (k / per / kStages) & 1, p.err);
-      }
-    }
-  } else if (warp == 1 && fit) {
-    if (elect_one()) {
-      constexpr uint32_t id_qk = idesc_f16(1, 1, 0, 0, kTreeRows, kTreeKeys);  // both K-major
-      constexpr uint32_t id_pv = idesc_f16(1, 1, 0, 1, kTreeRows, 256);        // V rows as they lie: MN-major
-      const uint64_t q_desc = smem_desc(s_base + OFF_Q, 16, 1024, LAYOUT_SW128);
-      const uint64_t k_desc = smem_desc(s_base + OFF_KV, 16, 1024, LAYOUT_SW128);
-      const uint64_t v_desc = smem_desc(s_base + OFF_KV, kBox, 1024, LAYOUT_SW128);
-      const uint64_t p_desc = smem_desc(s_base + OFF_P, 16, 1024, LAYOUT_SW128);
-      uint32_t g = 0;
-      bool ok = true;
-      for (int it = it0, n = 0; it < it1 && ok; ++it, ++n) {
-        const int t0 = p.items[it].tile0, t1 = p.items[it].tile1;
-        ok = mbar_wait(&B->q_full, n & 1, abort, p.err, ERR_TIMEOUT_FULL);
-        for (int t = t0; t < t1 && ok; ++t, ++g) {
-          const uint32_t st = g % kStages, par = (g / kStages) & 1, sb = g & 1;
-          const uint64_t kd = k_desc + (st * kStage >> 4), vd = v_desc + (st * kStage >> 4);
-          const uint32_t s_lat = tmem + kColS + sb * kSCols;
-          const uint32_t s_rope = s_lat + (Q8 ? 32 : 0);
-          // ---- S = Q . K^T
-          ok = mbar_wait(&B->s_empty[sb], ((g >> 1) & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY) &&
-               mbar_wait(&B->full[st][CH_ROPE], par, abort, p.err, ERR_TIMEOUT_FULL);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_f16_ws_ss(s_rope, q_desc + (8 * kBox + kk * 32) / 16, kd + (8 * kBox + kk * 32) / 16, id_qk, kk > 0);
-          for (int c = CH_LO; c <= CH_HI && ok; ++c) {
-            ok = mbar_wait(&B->full[st][c], par, abort, p.err, ERR_TIMEOUT_FULL);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t o = (c - 1) * (4 * kBox / 16);
-#pragma unroll
-            for (int k = 0; k < 16; ++k)
-              mma_f16_ws_ss(s_lat, q_desc + o + ((k >> 2) * kBox + (k & 3) * 32) / 16,
-                            kd + o + ((k >> 2) * kBox + (k & 3) * 32) / 16, id_qk,
-                            Q8 ? (c > CH_LO || k > 0) : 1u);
-          }
-          if (!ok) break;
-          mma_commit(&B->s_full[sb]);
-          mma_commit(&B->empty[st][CH_ROPE]);
-          if (t + 1 == t1) mma_commit(&B->q_empty);
-          // ---- O += P . V
-          ok = mbar_wait(&B->p_full, g & 1, abort, p.err, ERR_TIMEOUT_FULL);
-          if (ok && t == t0 && n > 0) ok = mbar_wait(&B->o_empty, (n - 1) & 1, abort, p.err, ERR_TIMEOUT_EMPTY);
-          if (!ok) break;
+    } else if (warp == 1 && fit) {
+      if (elect_one()) {
+        constexpr uint32_t id_qk = idesc_f16(1, 1, 0, 0, kTreeRows, kTreeKeys);  // both K-major
+        constexpr uint32_t id_pv = idesc_f16(1, 1, 0, 1, kTreeRows, 256);        // V rows as they lie: MN-major
+        const uint32_t k_lo = desc_lo(s_base, 16), v_lo = desc_lo(s_base, kBox);  // K-major boxes; MN-major, 64 dims a box
+        constexpr uint32_t kU16 = kUnit / 16, kB16 = kBox / 16;
+        uint32_t g = 0, u = 0;
+        bool ok = true;
+        // the tile whose P.V has not been issued yet
+        bool pend = false, pend_first = false;
+        uint32_t pend_u = 0;
+        int pend_n = 0;
+        auto pv = [&]() -> bool {  // O += P . V of tile g - 1
+          const uint32_t r = (g - 1) & 1;
+          if (!mbar_wait(&B->p_full, r, abort, p.err, ERR_TIMEOUT_FULL)) return false;
+          if (pend_first && pend_n > 0 && !mbar_wait(&B->o_empty, (pend_n - 1) & 1, abort, p.err, ERR_TIMEOUT_EMPTY))
+            return false;
           tc_fence_after();
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
+            const uint32_t s = (pend_u + h) % C::kUnits;
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              mma_f16_ws_ss(tmem + 128 * h, p_desc + kk * 2, vd + (h * 4 * kBox + kk * 2048) / 16, id_pv,
-                            t > t0 || kk > 0);
-            mma_commit(&B->empty[st][CH_LO + h]);
+              mma_f16_ws_ss(tmem + 128 * h, desc_of(k_lo + C::OFF_RP / 16 + r * kB16 + kk * 2),
+                            desc_of(v_lo + s * kU16 + kk * 128), id_pv, !pend_first || kk > 0);
+            mma_commit(&B->lat_empty[s]);
           }
+          mma_commit(&B->rp_empty[r]);
           mma_commit(&B->pv_done);
+          pend = false;
+          return true;
+        };
+        for (int it = it0, n = 0; it < it1 && ok; ++it, ++n) {
+          const int t0 = p.items[it].tile0, t1 = p.items[it].tile1;
+          // Q8: the first tile's second unit takes the place of the last tile's
+          // first one, which that tile's P.V frees
+          if (Q8 && pend) ok = pv();
+          // ---- the query's boxes to tensor memory, once the scores before have read theirs
+          if (ok && n > 0) ok = mbar_wait(&B->q_done, (n - 1) & 1, abort, p.err, ERR_TIMEOUT_MMA);
+          for (int h = 0; h < 2 && ok; ++h, ++u) {
+            const uint32_t s = u % C::kUnits;
+            ok = mbar_wait(&B->lat_full[s], (u / C::kUnits) & 1, abort, p.err, ERR_TIMEOUT_FULL);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int b = 0; b < (h ? C::kQT - 4 : 4); ++b)
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                tmem_cp_64x128b_x2(tmem + C::kColQ + 32 * (4 * h + b) + 4 * c, desc_of(k_lo + s * kU16 + b * kB16 + c));
+            mma_commit(&B->lat_empty[s]);
+          }
+          for (int t = t0; t < t1 && ok; ++t, ++g, u += 2) {
+            // The scores of this tile go before the P.V of the one before, which
+            // waits for its softmax -- unless this tile is still on its way.
+            if (pend && !mbar_test(&B->lat_full[(u + 1) % C::kUnits], ((u + 1) / C::kUnits) & 1)) ok = pv();
+            // ---- S = Q . K^T
+            if (ok) ok = mbar_wait(&B->s_empty, (g & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY);
+            const uint32_t s_lat = tmem + C::kColS, s_rope = s_lat + (Q8 ? 32 : 0);
+            // opaque, or the compiler keeps all 36 operand addresses in registers across tiles
+            uint32_t tq = tmem + C::kColQ, kl = k_lo;
+            asm volatile("" : "+r"(tq), "+r"(kl));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t s = (u + h) % C::kUnits;
+              if (ok) ok = mbar_wait(&B->lat_full[s], ((u + h) / C::kUnits) & 1, abort, p.err, ERR_TIMEOUT_FULL);
+              if (ok && h && t == t0) ok = mbar_wait(&B->qs_full, n & 1, abort, p.err, ERR_TIMEOUT_FULL);
+              if (!ok) break;
+              tc_fence_after();
+#pragma unroll
+              for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {
+                  const uint64_t kd = desc_of(kl + s * kU16 + b * kB16 + kk * 2);
+                  const int qb = 4 * h + b;
+                  if (qb < C::kQT)
+                    mma_f16_ws_ts(s_lat, tq + 32 * qb + 8 * kk, kd, id_qk, qb + kk > 0);
+                  else
+                    mma_f16_ws_ss(s_lat, desc_of(kl + C::OFF_QS / 16 + (qb - C::kQT) * kB16 + kk * 2), kd, id_qk, 1u);
+                }
+            }
+            if (ok) ok = mbar_wait(&B->rp_full[g & 1], (g >> 1) & 1, abort, p.err, ERR_TIMEOUT_FULL);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_f16_ws_ss(s_rope, desc_of(kl + C::OFF_QS / 16 + (8 - C::kQT) * kB16 + kk * 2),
+                            desc_of(kl + C::OFF_RP / 16 + (g & 1) * kB16 + kk * 2), id_qk, Q8 ? kk > 0 : 1u);
+            mma_commit(&B->s_full);
+            if (t + 1 == t1) mma_commit(&B->q_done);
+            if (pend) ok = pv();
+            pend = true;
+            pend_first = t == t0;
+            pend_u = u;
+            pend_n = n;
+          }
         }
+        if (ok && pend) pv();
+        // issued tensor-core work ends before tensor memory is released
+        mma_commit(&B->drain);
+        drain_wait(&B->drain, 0, p.err);
       }
-      // issued tensor-core work ends before tensor memory is released
-      mma_commit(&B->drain);
-      drain_wait(&B->drain, 0, p.err);
-    }
-  } else if (warp == 2 && fit) {
-    if (elect_one()) {
-      tma_prefetch_desc(&p.tm_q);
-      bool ok = true;
-      int n = 0;
-      for (int it = it0; it < it1; ++it, ++n) {
-        const int node0 = p.items[it].node0;
-        if (n > 0) ok = mbar_wait(&B->q_empty, (n - 1) & 1, abort, p.err, ERR_TIMEOUT_EMPTY);
-        if (!ok) break;
-        mbar_arrive_expect_tx(&B->q_full, kBoxes * kBox);
-        for (int b = 0; b < kBoxes; ++b)
-          tma_load_2d(smem + OFF_Q + b * kBox, &p.tm_q, &B->q_full, 64 * b, node0 * kHeads);
+    } else if (warp == 2 && fit) {
+      if (elect_one()) {
+        bool ok = true;
+        int n = 0;
+        for (int it = it0; it < it1; ++it, ++n) {
+          const int node0 = p.items[it].node0;
+          if (n > 0) ok = mbar_wait(&B->q_done, (n - 1) & 1, abort, p.err, ERR_TIMEOUT_EMPTY);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&B->qs_full, C::kQS * kBox);
+          for (int b = 0; b < C::kQS; ++b)
+            tma_load_2d(smem + C::OFF_QS + b * kBox, &p.tm_q, &B->qs_full, 64 * (C::kQT + b), node0 * kHeads);
+        }
+        if (!ok) drain_wait(&B->qs_full, (n - 1) & 1, p.err);
       }
-      if (!ok) drain_wait(&B->q_full, (n - 1) & 1, p.err);
     }
-  } else if (warp >= 4 && warp < 8 && fit) {
-    const int tid = threadIdx.x - 128;
-    const int row = tid & 63, half = tid >> 6;
-    const uint32_t lanes = static_cast<uint32_t>(32 * (warp - 4)) << 16;
-    uint32_t g = 0;
-    bool bad = false;
-    for (int it = it0; it < it1 && !bad; ++it) {
-      const TreeItem im = p.items[it];
-      const bool real = row < im.nn * kHeads;
-      uint64_t mask = real ? p.mask[im.node0 + row / kHeads] : 0;
-      if (im.tree < 64) mask &= (uint64_t(1) << im.tree) - 1;
-      float m = -INFINITY, l = 0.f;
-      for (int t = im.tile0; t < im.tile1; ++t, ++g) {
-        const uint32_t st = g % kStages, sb = g & 1;
-        bad |= !mbar_wait(&B->s_full[sb], (g >> 1) & 1, abort, p.err, ERR_TIMEOUT_MMA);
-        if (Q8) bad |= !mbar_wait(&B->full[st][CH_HI], (g / kStages) & 1, abort, p.err, ERR_TIMEOUT_FULL);
-        tc_fence_after();
-        float s[32], sr[Q8 ? 32 : 1];
-        tmem_ld32(tmem + kColS + sb * kSCols + lanes, s);
-        if (Q8) tmem_ld32(tmem + kColS + sb * kSCols + 32 + lanes, sr);
-        tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&B->s_empty[sb]);
-        const float *ks = B->scale[st] + 32 * half;
-        const int k0 = kTreeKeys * t + 32 * half;  // the thread's first key
-        uint32_t seen = 0xffffffffu;
-        if (Q8)
+  } else if (warp < 8) {
+    if (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+    if (fit) {
+      const int tid = threadIdx.x - 128;
+      const int row = tid & 63, half = tid >> 6;
+      const uint32_t lanes = static_cast<uint32_t>(32 * (warp - 4)) << 16;
+      uint32_t g = 0, u = 0;
+      bool bad = false;
+      for (int it = it0; it < it1 && !bad; ++it) {
+        const TreeItem im = p.items[it];
+        u += 2;  // its query
+        const bool real = row < im.nn * kHeads;
+        uint64_t mask = real ? p.mask[im.node0 + row / kHeads] : 0;
+        if (im.tree < 64) mask &= (uint64_t(1) << im.tree) - 1;
+        float m = -INFINITY, l = 0.f;
+        for (int t = im.tile0; t < im.tile1; ++t, ++g, u += 2) {
+          bad |= !mbar_wait(&B->s_full, g & 1, abort, p.err, ERR_TIMEOUT_MMA);
+          const float *ks = B->scale[g % kScaleRing] + 32 * half;
+          if (Q8)  // the converters' row scales
+            bad |= !mbar_wait(&B->lat_full[(u + 1) % C::kUnits], ((u + 1) / C::kUnits) & 1, abort, p.err,
+                              ERR_TIMEOUT_FULL);
+          tc_fence_after();
+          float s[32];
+          tmem_ld32(tmem + C::kColS + lanes, s);
+          tmem_wait_ld();
+          if (Q8) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c) s[c] = fmaf(s[c], ks[c], sr[c]);
-        const bool masked = kTreeKeys * (t + 1) > im.len;
-        if (masked) {
-          const int d = k0 - im.len;  // drafted row of the first key
-          seen = d >= 0 ? (d < 64 ? static_cast<uint32_t>(mask >> d) : 0u)
-                        : (d > -32 ? static_cast<uint32_t>(mask << -d) | (0xffffffffu >> (32 + d)) : 0xffffffffu);
-          if (!Q8) {
-            // A hidden row gets p = 0, but 0 times an infinity or a NaN of the
-            // row itself is NaN in the P.V product.  Such a row gives a score
-            // that is not finite with every query (a query that is not finite
-            // does so with every row, but only its own): clear those rows.
-            uint32_t nf = 0;
+            for (int i = 0; i < 32; i += 16) {
+              float sr[16];
+              tmem_ld16(tmem + C::kColS + 32 + i + lanes, sr);
+              tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 32; ++c) nf |= ((__float_as_uint(s[c]) & 0x7f800000u) == 0x7f800000u) ? 1u << c : 0u;
-            if (named_bar_or(2, 128, (nf & ~seen) != 0)) {
-              const uint32_t all = __reduce_and_sync(0xffffffffu, nf);
-              if (lane == 0) B->nonfinite[warp - 4] = all;
-              named_bar_sync(2, 128);
-              const uint64_t rows = static_cast<uint64_t>(B->nonfinite[0] & B->nonfinite[1]) |
-                                    static_cast<uint64_t>(B->nonfinite[2] & B->nonfinite[3]) << 32;
-              uint8_t *v = smem + OFF_KV + st * kStage + (tid >> 3 & 7) * kBox + (tid & 7) * 16;
-              for (int k = tid >> 6; k < kTreeKeys; k += 2)
-                if (rows >> k & 1) *reinterpret_cast<uint4 *>(v + k * 128) = make_uint4(0u, 0u, 0u, 0u);
+              for (int c = 0; c < 16; ++c) s[i + c] = fmaf(s[i + c], ks[i + c], sr[c]);
             }
           }
-        }
-        float mx = -INFINITY;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&B->s_empty);
+          const int k0 = kTreeKeys * t + 32 * half;  // the thread's first key
+          uint32_t seen = 0xffffffffu;
+          const bool masked = kTreeKeys * (t + 1) > im.len;
+          if (masked) {
+            const int d = k0 - im.len;  // drafted row of the first key
+            seen = d >= 0 ? (d < 64 ? static_cast<uint32_t>(mask >> d) : 0u)
+                          : (d > -32 ? static_cast<uint32_t>(mask << -d) | (0xffffffffu >> (32 + d)) : 0xffffffffu);
+            if (!Q8) {
+              // A hidden row gets p = 0, but 0 times an infinity or a NaN of the
+              // row itself is NaN in the P.V product.  Such a row gives a score
+              // that is not finite with every query (a query that is not finite
+              // does so with every row, but only its own): clear those rows.
+              uint32_t nf = 0;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          s[c] = (seen >> c & 1) ? s[c] * p.scale_log2 : -INFINITY;
-          mx = fmaxf(mx, s[c]);
+              for (int c = 0; c < 32; ++c) nf |= ((__float_as_uint(s[c]) & 0x7f800000u) == 0x7f800000u) ? 1u << c : 0u;
+              if (named_bar_or(2, 128, (nf & ~seen) != 0)) {
+                const uint32_t all = __reduce_and_sync(0xffffffffu, nf);
+                if (lane == 0) B->nonfinite[warp - 4] = all;
+                named_bar_sync(2, 128);
+                const uint64_t rows = static_cast<uint64_t>(B->nonfinite[0] & B->nonfinite[1]) |
+                                      static_cast<uint64_t>(B->nonfinite[2] & B->nonfinite[3]) << 32;
+                const uint32_t box = tid >> 3 & 7;
+                uint8_t *v = smem + ((u + (box >> 2)) % C::kUnits) * kUnit + (box & 3) * kBox + (tid & 7) * 16;
+                for (int k = tid >> 6; k < kTreeKeys; k += 2)
+                  if (rows >> k & 1) *reinterpret_cast<uint4 *>(v + k * 128) = make_uint4(0u, 0u, 0u, 0u);
+              }
+            }
+          }
+          float mx = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            s[c] = (seen >> c & 1) ? s[c] * p.scale_log2 : -INFINITY;
+            mx = fmaxf(mx, s[c]);
+          }
+          // the other half of the row's keys
+          B->red[g & 1][tid] = mx;
+          if (named_bar_or(1, 128, bad)) {
+            bad = true;
+            break;
+          }
+          mx = fmaxf(mx, B->red[g & 1][tid ^ 64]);
+          // The reference maximum moves only when a score exceeds it by 2^8; both
+          // warps of a row decide alike.
+          if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
+            const float mn = fmaxf(m, mx);
+            const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
+            if (t > im.tile0) {
+              bad |= !mbar_wait(&B->pv_done, (g - 1) & 1, abort, p.err, ERR_TIMEOUT_MMA);
+              tc_fence_after();
+#pragma unroll
+              for (int c = 0; c < 256; c += 32) {
+                float o[32];
+                tmem_ld32(tmem + c + lanes, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] *= alpha;
+                tmem_st32(tmem + c + lanes, o);
+              }
+              tmem_wait_st();
+            }
+            l *= alpha;
+            m = mn;
+          }
+          const float ref = m == -INFINITY ? 0.f : m;  // a row that has seen nothing: exp2(-inf) = 0
+          uint32_t pk[16];
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            float p0 = ex2(s[c] - ref), p1 = ex2(s[c + 1] - ref);
+            l += p0 + p1;
+            if (Q8) {  // O accumulates p * scale * int8 row; a hidden row's scale may be anything
+              p0 = (seen >> c & 1) ? p0 * ks[c] : 0.f;
+              p1 = (seen >> (c + 1) & 1) ? p1 * ks[c + 1] : 0.f;
+            }
+            pk[c / 2] = pack_bf16(p0, p1);
+          }
+          // in the place of the tile's rope, which the scores have read
+          uint8_t *pd = smem + C::OFF_RP + (g & 1) * kBox + (row >> 3) * 1024 + (row & 7) * 128;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<uint4 *>(pd + ((4 * half + c) ^ (row & 7)) * 16) =
+                make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+          fence_proxy_async_smem();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&B->p_full);
         }
-        // the other half of the row's keys
-        B->red[sb][tid] = mx;
+        if (bad) break;
+        // ---- epilogue
+        bad |= !mbar_wait(&B->pv_done, (g - 1) & 1, abort, p.err, ERR_TIMEOUT_MMA);
+        B->red[2][tid] = l;
         if (named_bar_or(1, 128, bad)) {
           bad = true;
           break;
         }
-        mx = fmaxf(mx, B->red[sb][tid ^ 64]);
-        // The reference maximum moves only when a score exceeds it by 2^8; both
-        // warps of a row decide alike.
-        if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
-          const float mn = fmaxf(m, mx);
-          const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
-          if (t > im.tile0) {
-            bad |= !mbar_wait(&B->pv_done, (g - 1) & 1, abort, p.err, ERR_TIMEOUT_MMA);
-            tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < 256; c += 32) {
-              float o[32];
-              tmem_ld32(tmem + c + lanes, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] *= alpha;
-              tmem_st32(tmem + c + lanes, o);
-            }
-            tmem_wait_st();
-          }
-          l *= alpha;
-          m = mn;
+        tc_fence_after();
+        l += B->red[2][tid ^ 64];
+        const float inv = l == 0.f ? 0.f : 1.0f / l;  // nothing seen: out = 0, lse = -inf
+        if (real && half == 0) {
+          const float lse = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+          if (im.slot >= 0)
+            p.part_lse[static_cast<size_t>(im.slot) * kTreeRows + row] = lse;
+          else if (p.lse)
+            p.lse[static_cast<size_t>(im.node0) * kHeads + row] = lse;
         }
-        const float ref = m == -INFINITY ? 0.f : m;  // a row that has seen nothing: exp2(-inf) = 0
-        uint32_t pk[16];
+        // A partial keeps the threads' own layout, [64 column quads][128 threads]
+        // float4: every store of a warp is 512 contiguous bytes.  (Row by row,
+        // 16 bytes of 32 different rows a store, an item's end took 13000 cycles.)
+        float4 *part = reinterpret_cast<float4 *>(p.part_o) + (static_cast<size_t>(max(im.slot, 0)) * 64) * 128 + tid;
+        uint16_t *orow = p.out + (static_cast<size_t>(im.node0) * kHeads + row) * kLatent + half * 128;
 #pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          float p0 = ex2(s[c] - ref), p1 = ex2(s[c + 1] - ref);
-          l += p0 + p1;
-          if (Q8) {  // O accumulates p * scale * int8 row; a hidden row's scale may be anything
-            p0 = (seen >> c & 1) ? p0 * ks[c] : 0.f;
-            p1 = (seen >> (c + 1) & 1) ? p1 * ks[c + 1] : 0.f;
-          }
-          pk[c / 2] = pack_bf16(p0, p1);
-        }
-        // P of the tile before is read until its P.V ends
-        if (g > 0) bad |= !mbar_wait(&B->pv_done, (g - 1) & 1, abort, p.err, ERR_TIMEOUT_MMA);
-        uint8_t *pd = smem + OFF_P + (row >> 3) * 1024 + (row & 7) * 128;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          *reinterpret_cast<uint4 *>(pd + ((4 * half + c) ^ (row & 7)) * 16) =
-              make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
-        fence_proxy_async_smem();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&B->p_full);
-      }
-      if (bad) break;
-      // ---- epilogue
-      bad |= !mbar_wait(&B->pv_done, (g - 1) & 1, abort, p.err, ERR_TIMEOUT_MMA);
-      B->red[2][tid] = l;
-      if (named_bar_or(1, 128, bad)) {
-        bad = true;
-        break;
-      }
-      tc_fence_after();
-      l += B->red[2][tid ^ 64];
-      const float inv = l == 0.f ? 0.f : 1.0f / l;  // nothing seen: out = 0, lse = -inf
-      if (real && half == 0) {
-        const float lse = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
-        if (im.slot >= 0)
-          p.part_lse[static_cast<size_t>(im.slot) * kTreeRows + row] = lse;
-        else if (p.lse)
-          p.lse[static_cast<size_t>(im.node0) * kHeads + row] = lse;
-      }
-      const size_t orow = im.slot >= 0 ? static_cast<size_t>(im.slot) * kTreeRows + row
-                                       : static_cast<size_t>(im.node0) * kHeads + row;
-#pragma unroll
-      for (int c = 0; c < 256; c += 32) {
-        float o[32];
-        tmem_ld32(tmem + c + lanes, o);
-        tmem_wait_ld();
-        const int d = (c >> 7) * 256 + half * 128 + (c & 127);
-        if (real) {
+        for (int c = 0; c < 256; c += 32) {
+          float o[32];
+          tmem_ld32(tmem + c + lanes, o);
+          tmem_wait_ld();
           if (im.slot >= 0) {
-            float4 *dst = reinterpret_cast<float4 *>(p.part_o + orow * kLatent + d);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              dst[i] = make_float4(o[4 * i] * inv, o[4 * i + 1] * inv, o[4 * i + 2] * inv, o[4 * i + 3] * inv);
-          } else {
-            uint4 *dst = reinterpret_cast<uint4 *>(p.out + orow * kLatent + d);
+              part[(c / 4 + i) * 128] =
+                  make_float4(o[4 * i] * inv, o[4 * i + 1] * inv, o[4 * i + 2] * inv, o[4 * i + 3] * inv);
+          } else if (real) {
+            uint4 *dst = reinterpret_cast<uint4 *>(orow + (c >> 7) * 256 + (c & 127));
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               dst[i] = make_uint4(pack_bf16(o[8 * i] * inv, o[8 * i + 1] * inv),
@@ -616,12 +762,12 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
                                   pack_bf16(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
           }
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B->o_empty);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&B->o_empty);
     }
-  } else if (Q8 && warp >= kConvertWarp && fit) {
+  } else if (Q8 && fit) {
     // Thread t has the 16 latents c = t % 4 of row t / 4 in each of the eight
     // boxes: four threads read 64 consecutive bytes, and the eight lanes of a
     // store phase (two rows) fill the eight 16-byte banks of the swizzle.
@@ -631,15 +777,22 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
     // the CTA's tiles in order
     int it = it0, t = it0 < it1 ? p.items[it0].tile0 : 0, t1 = it0 < it1 ? p.items[it0].tile1 : 0;
     long long row0 = it0 < it1 ? p.items[it0].row0 : 0;
-    auto load = [&](uint4(&v)[8], float &sc) -> bool {
-      while (it < it1 && t >= t1) {
+    uint32_t u = 0, u0 = 0, u1 = 0;  // units of the ring so far; of the tiles in v0 and v1
+    bool fresh = true;               // the next tile is its item's first: two query units come before it
+    auto load = [&](uint4(&v)[8], float &sc, uint32_t &un) -> bool {
+      if (it < it1 && t >= t1) {
         if (++it < it1) {
           t = p.items[it].tile0;
           t1 = p.items[it].tile1;
           row0 = p.items[it].row0;
+          fresh = true;
         }
       }
       if (it >= it1) return false;
+      if (fresh) u += 2;
+      fresh = false;
+      un = u;
+      u += 2;
       const long long first = row0 + static_cast<long long>(kTreeKeys) * t;
       const uint4 *src = reinterpret_cast<const uint4 *>(p.lat8 + min(first + r, last) * kLatent) + c;
 #pragma unroll
@@ -649,37 +802,37 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
       return true;
     };
     uint32_t g = 0;
-    auto store = [&](const uint4(&v)[8], float sc) -> bool {
-      const uint32_t st = g % kStages, par = ((g / kStages) & 1) ^ 1;
-      uint8_t *dst = smem + OFF_KV + st * kStage + (r >> 3) * 1024 + (r & 7) * 128;
+    auto store = [&](const uint4(&v)[8], float sc, uint32_t un) -> bool {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (!mbar_wait(&B->empty[st][CH_LO + h], par, abort, p.err, ERR_TIMEOUT_EMPTY)) return false;
-        if (h == 1 && tid < kTreeKeys) B->scale[st][tid] = sc;
+        const uint32_t slot = (un + h) % C::kUnits;
+        if (!mbar_wait(&B->lat_empty[slot], (((un + h) / C::kUnits) & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY))
+          return false;
+        uint8_t *dst = smem + slot * kUnit + (r >> 3) * 1024 + (r & 7) * 128;
+        if (h == 1 && tid < kTreeKeys) B->scale[g % kScaleRing][tid] = sc;
 #pragma unroll
-        for (int b = 4 * h; b < 4 * h + 4; ++b) {
+        for (int b = 0; b < 4; ++b) {
+          const uint4 x = v[4 * h + b];
           *reinterpret_cast<uint4 *>(dst + b * kBox + ((2 * c) ^ (r & 7)) * 16) =
-              make_uint4(s8x2_to_bf16<0>(v[b].x), s8x2_to_bf16<1>(v[b].x), s8x2_to_bf16<0>(v[b].y),
-                         s8x2_to_bf16<1>(v[b].y));
+              make_uint4(s8x2_to_bf16<0>(x.x), s8x2_to_bf16<1>(x.x), s8x2_to_bf16<0>(x.y), s8x2_to_bf16<1>(x.y));
           *reinterpret_cast<uint4 *>(dst + b * kBox + ((2 * c + 1) ^ (r & 7)) * 16) =
-              make_uint4(s8x2_to_bf16<0>(v[b].z), s8x2_to_bf16<1>(v[b].z), s8x2_to_bf16<0>(v[b].w),
-                         s8x2_to_bf16<1>(v[b].w));
+              make_uint4(s8x2_to_bf16<0>(x.z), s8x2_to_bf16<1>(x.z), s8x2_to_bf16<0>(x.w), s8x2_to_bf16<1>(x.w));
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&B->full[st][CH_LO + h]);
+        if (lane == 0) mbar_arrive(&B->lat_full[slot]);
       }
       ++g;
       return true;
     };
     uint4 v0[8], v1[8];
     float sc0 = 0.f, sc1 = 0.f;
-    bool more = load(v0, sc0);
+    bool more = load(v0, sc0, u0);
     while (more) {  // the next tile's rows are in flight while this one is stored
-      const bool second = load(v1, sc1);
-      if (!store(v0, sc0) || !second) break;
-      more = load(v0, sc0);
-      if (!store(v1, sc1)) break;
+      const bool second = load(v1, sc1, u1);
+      if (!store(v0, sc0, u0) || !second) break;
+      more = load(v0, sc0, u0);
+      if (!store(v1, sc1, u1)) break;
     }
   }
 
@@ -695,51 +848,96 @@ cudaError_t launch_tree_attend(const TreeParams &p, bool q8, int grid, cudaStrea
   static std::atomic<unsigned long long> opted[2];
   const void *fn = q8 ? reinterpret_cast<const void *>(tree_attend_kernel<true>)
                       : reinterpret_cast<const void *>(tree_attend_kernel<false>);
-  cudaError_t e = smem_opt_in(fn, kSmemBytes, opted[q8]);
+  cudaError_t e = smem_opt_in(fn, q8 ? smem_bytes<true>() : smem_bytes<false>(), opted[q8]);
   if (e != cudaSuccess) return e;
   ProfScope ps(q8 ? "tree_attend_q8" : "tree_attend_bf16", s);
   if (q8)
-    tree_attend_kernel<true><<<grid, threads<true>(), kSmemBytes, s>>>(p);
+    tree_attend_kernel<true><<<grid, threads<true>(), smem_bytes<true>(), s>>>(p);
   else
-    tree_attend_kernel<false><<<grid, threads<false>(), kSmemBytes, s>>>(p);
+    tree_attend_kernel<false><<<grid, threads<false>(), smem_bytes<false>(), s>>>(p);
   return cudaGetLastError();
 }
 
-// One block per (entry, query row, 128 dims): the partials of a split chunk
-// range, combined as merge_core.cuh does, written as bf16.
-__global__ void tree_merge_kernel(uint16_t *out, float *lse, const float *part_o, const float *part_lse,
-                                  const TreeMerge *entries) {
-  const int row = blockIdx.y;
+// Combines the partials of the split (sequence, group)s:
+//     out = sum_q w_q o_q / sum_q w_q,  w_q = exp(lse_q - max lse),
+//     lse = max lse + log sum_q w_q.
+// Thread (tid, z) of block (entry, quad) has four output dims of one query row,
+// as the attend's thread tid left them, and the parts z, z + Z, ...; the Z
+// sums are added in order.  Bound by reading the partials (L2 mostly).
+template <int Z>
+__global__ void __launch_bounds__(128 * Z) tree_merge_kernel(uint16_t *out, float *lse, const float *part_o,
+                                                             const float *part_lse, const TreeMerge *entries) {
   const TreeMerge e = entries[blockIdx.x];
+  const int tid = threadIdx.x & 127, z = threadIdx.x >> 7, quad = blockIdx.y;
+  const int row = tid & 63, half = tid >> 6;
+  __shared__ float4 acc_z[Z > 1 ? Z : 1][128];
+  __shared__ float max_z[Z][128], sum_z[Z][128];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (row >= e.nn * kHeads) return;
-  const MergeSlice r = merge_slice(MergeEntry{0, e.first, e.count, 1}, row, blockIdx.z, part_o, part_lse, kTreeRows,
-                                   kLatent, 1, static_cast<long long>(kTreeRows) * kLatent, kTreeRows, true);
-  const size_t orow = static_cast<size_t>(e.node0) * kHeads + row;
-  const bool none = r.m == -INFINITY;  // no part has seen a row
-  if (lse && blockIdx.z == 0 && threadIdx.x == 0) lse[orow] = none ? -INFINITY : r.m + logf(r.sum);
-  if (threadIdx.x < 32) {
-    const float inv = 1.0f / r.sum;
-    uint2 v = make_uint2(pack_bf16(r.t.x * inv, r.t.y * inv), pack_bf16(r.t.z * inv, r.t.w * inv));
-    if (none) v = make_uint2(0u, 0u);
-    *reinterpret_cast<uint2 *>(out + orow * kLatent + r.d0) = v;
+  const bool real = row < e.nn * kHeads;
+  const float *ls = part_lse + static_cast<size_t>(e.first) * kTreeRows + row;
+  const float4 *os = reinterpret_cast<const float4 *>(part_o) + (static_cast<size_t>(e.first) * 64 + quad) * 128 + tid;
+  float m = -INFINITY;
+  if (real)
+    for (int q = z; q < e.count; q += Z) m = fmaxf(m, ls[q * kTreeRows]);
+  if (Z > 1) {
+    max_z[z][tid] = m;
+    __syncthreads();
+    for (int i = 0; i < Z; ++i) m = fmaxf(m, max_z[i][tid]);
   }
+  const float ref = m == -INFINITY ? 0.f : m;  // no part has seen a row: all weights are 0
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  if (real) {
+#pragma unroll 4
+    for (int q = z; q < e.count; q += Z) {
+      const float w = __expf(ls[q * kTreeRows] - ref);
+      const float4 v = os[static_cast<size_t>(q) * 64 * 128];
+      sum += w;
+      acc.x = fmaf(w, v.x, acc.x);
+      acc.y = fmaf(w, v.y, acc.y);
+      acc.z = fmaf(w, v.z, acc.z);
+      acc.w = fmaf(w, v.w, acc.w);
+    }
+  }
+  if (Z > 1) {
+    acc_z[z][tid] = acc;
+    sum_z[z][tid] = sum;
+    __syncthreads();
+    if (z > 0) return;
+    for (int i = 1; i < Z; ++i) {
+      const float4 v = acc_z[i][tid];
+      acc.x += v.x;
+      acc.y += v.y;
+      acc.z += v.z;
+      acc.w += v.w;
+      sum += sum_z[i][tid];
+    }
+  }
+  if (!real) return;
+  const size_t orow = static_cast<size_t>(e.node0) * kHeads + row;
+  if (lse && quad == 0 && half == 0) lse[orow] = sum == 0.f ? -INFINITY : m + logf(sum);
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  const int c = 4 * quad;  // the attend thread's column
+  *reinterpret_cast<uint2 *>(out + orow * kLatent + (c >> 7) * 256 + half * 128 + (c & 127)) =
+      make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
 }
 
 cudaError_t launch_tree_merge(const TreeParams &p, const TreeMerge *entries, int n, int max_count, cudaStream_t s) {
   if (n <= 0) return cudaSuccess;
   ProfScope ps("tree_merge", s);
+  // a few parts a thread: more threads share an entry that has many
+  const int z = max_count <= 8 ? 1 : max_count <= 32 ? 4 : 8;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(n, kTreeRows, kLatent / 128);
-  cfg.blockDim = dim3(32 * merge_warps(max_count));
+  cfg.gridDim = dim3(n, 64);
+  cfg.blockDim = dim3(128 * z);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, tree_merge_kernel, p.out, p.lse, (const float *)p.part_o, (const float *)p.part_lse,
-                            entries);
+  auto f = z == 1 ? tree_merge_kernel<1> : z == 4 ? tree_merge_kernel<4> : tree_merge_kernel<8>;
+  return cudaLaunchKernelEx(&cfg, f, p.out, p.lse, (const float *)p.part_o, (const float *)p.part_lse, entries);
 }
 
 }  // namespace kvl
