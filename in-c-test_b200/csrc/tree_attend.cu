@@ -306,8 +306,9 @@ template <bool Q8>
 struct Cfg {
   static constexpr int kUnits = Q8 ? 5 : 6;
   static constexpr int kQT = Q8 ? 6 : 7, kQS = 9 - kQT;
-  static constexpr uint32_t OFF_RP = kUnits * kUnit;         // rope of a tile, then its P: two boxes
-  static constexpr uint32_t OFF_QS = OFF_RP + 2 * kBox;
+  static constexpr uint32_t OFF_R = kUnits * kUnit;  // a tile's rope, until its scores are done
+  static constexpr uint32_t OFF_P = OFF_R + kBox;    // a tile's P, until its P.V is
+  static constexpr uint32_t OFF_QS = OFF_P + kBox;
   static constexpr uint32_t OFF_BAR = OFF_QS + kQS * kBox;
   // O (64 rows x 512) takes 256 columns: dims [256 i, 256 i + 128) in columns
   // [128 i, 128 i + 128) of lanes 0-63, the next 128 dims in lanes 64-127.
@@ -315,14 +316,17 @@ struct Cfg {
   static_assert(kColQ + 32 * kQT == 512, "tensor memory");
 };
 constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kU16 = kUnit / 16, kB16 = kBox / 16;  // in units of a matrix descriptor
 constexpr int kScaleRing = 4;
 
 struct Bars {
-  uint64_t lat_full[6], lat_empty[6];
-  uint64_t rp_full[2], rp_empty[2];  // empty: the tile's P.V is done
-  uint64_t qs_full, q_done;          // q_done: the item's last scores are done
+  // of step j: [j % 4], phase j / 4.  full: its latents are there; done: its P.V
+  // (its copy to tensor memory) is, so its place is free
+  uint64_t full[4], done[4];
+  uint64_t rope_full;
+  uint64_t qs_full, q_done;  // q_done: the item's last scores are done
   uint64_t s_full, s_empty;
-  uint64_t p_full, pv_done, o_empty, drain;
+  uint64_t p_full, o_empty, drain[2];
   uint32_t tmem_base;
   int abort;
   uint32_t nonfinite[4];
@@ -370,17 +374,26 @@ __device__ __forceinline__ uint32_t s8x2_to_bf16(uint32_t w) {
 
 using namespace treek;
 
+// Waits until step `k` is done.  Steps share four barriers, so nobody may ask
+// for a step that is four or more behind the last one loaded.
+__device__ __forceinline__ bool wait_done(Bars *B, uint32_t k, volatile int *abort, uint32_t *err) {
+  return mbar_wait(&B->done[k & 3], (k >> 2) & 1, abort, err, ERR_TIMEOUT_EMPTY);
+}
+
 // One CTA per SM, roles by warp:
 //   0      TMA producer: queries, ropes, bf16 latents
-//   1      tcgen05 issuer
+//   1, 3   tcgen05 issuers, of the scores and of P.V: a commit holds its thread
+//          until the MMAs before it have left the queue, so one thread for both
+//          leaves the tensor core idle 500 of a tile's 2150 cycles
 //   2      loader of the query boxes that stay in shared memory
 //   4-7    softmax and epilogue: thread t has query row t % 64 and keys
 //          32 (t / 64) .. + 31 of a tile (where .ws puts them)
 //   8-15   Q8: latents from global memory, as bf16 into the ring
 //
-// The latent ring runs in units of half a tile.  An item starts with two units
-// of query boxes, which the issuer copies to tensor memory (tcgen05.cp).  A
-// tile's rope box is read by the scores only; its P then takes the same place.
+// The latent ring runs in steps of two units, half a tile each.  An item is a
+// step of query boxes, which the issuer copies to tensor memory (tcgen05.cp),
+// then one step a tile.  The rope box has one place: it is loaded when the
+// scores before are done, from L2, where it was brought with the latents.
 template <bool Q8>
 __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __grid_constant__ TreeParams p) {
   using C = Cfg<Q8>;
@@ -393,22 +406,19 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
   volatile int *abort = &B->abort;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 6; ++i) {
-      mbar_init(&B->lat_full[i], Q8 ? kConvertThreads / 32 : 1);
-      mbar_init(&B->lat_empty[i], 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&B->full[i], Q8 ? kConvertThreads / 32 : 1);
+      mbar_init(&B->done[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&B->rp_full[i], 1);
-      mbar_init(&B->rp_empty[i], 1);
-    }
+    mbar_init(&B->rope_full, 1);
     mbar_init(&B->qs_full, 1);
     mbar_init(&B->q_done, 1);
     mbar_init(&B->s_full, 1);
     mbar_init(&B->s_empty, 4);
     mbar_init(&B->p_full, 4);
-    mbar_init(&B->pv_done, 1);
     mbar_init(&B->o_empty, 4);
-    mbar_init(&B->drain, 1);
+    mbar_init(&B->drain[0], 1);
+    mbar_init(&B->drain[1], 1);
     B->abort = 0;
     if (s_base & 1023) {  // the swizzle atoms
       B->abort = 1;
@@ -434,151 +444,156 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
       if (elect_one()) {
         tma_prefetch_desc(&p.tm_q);
         tma_prefetch_desc(&p.tm_kv);
-        uint32_t g = 0, u = 0, rp = 0;  // u: units of the ring so far, rp: ropes issued
+        uint32_t g = 0, j = 0;
         bool ok = true;
+        // the places of step j: their last steps must be done
+        auto free_unit = [&](int h) -> bool {
+          const uint32_t u = 2 * j + h;
+          return u < C::kUnits || wait_done(B, (u - C::kUnits) >> 1, abort, p.err);
+        };
+        TreeItem nx = p.items[it0];  // descriptors are read one item ahead
         for (int it = it0; it < it1 && ok; ++it) {
-          const TreeItem im = p.items[it];
-          for (int h = 0; h < 2 && ok; ++h, ++u) {
-            const uint32_t s = u % C::kUnits;
-            ok = mbar_wait(&B->lat_empty[s], ((u / C::kUnits) & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY);
+          const TreeItem im = nx;
+          if (it + 1 < it1) nx = p.items[it + 1];
+          uint64_t *full = &B->full[j & 3];
+          for (int h = 0; h < 2 && ok; ++h) {
+            ok = free_unit(h);
             if (!ok) break;
-            const int n = h ? C::kQT - 4 : 4;
-            mbar_arrive_expect_tx(&B->lat_full[s], n * kBox);
-            for (int b = 0; b < n; ++b)
-              tma_load_2d(smem + s * kUnit + b * kBox, &p.tm_q, &B->lat_full[s], 64 * (4 * h + b), im.node0 * kHeads);
-            if (Q8)  // the barrier counts the converter warps
-              for (int i = 1; i < kConvertThreads / 32; ++i) mbar_arrive(&B->lat_full[s]);
+            if (h == 0) mbar_arrive_expect_tx(full, C::kQT * kBox);
+            for (int b = 4 * h; b < (h ? C::kQT : 4); ++b)
+              tma_load_2d(smem + ((2 * j + h) % C::kUnits) * kUnit + (b & 3) * kBox, &p.tm_q, full, 64 * b,
+                          im.node0 * kHeads);
           }
-          for (int t = im.tile0; t < im.tile1 && ok; ++t, ++g) {
+          if (!ok) break;
+          if (Q8)  // the barrier counts the converter warps too
+            for (int i = 1; i < kConvertThreads / 32; ++i) mbar_arrive(full);
+          ++j;
+          for (int t = im.tile0; t < im.tile1 && ok; ++t, ++g, ++j) {
             const int32_t y = static_cast<int32_t>(im.row0 + static_cast<long long>(kTreeKeys) * t);
-            for (int h = 0; h < 2 && ok; ++h, ++u) {
-              if (Q8) continue;
-              const uint32_t s = u % C::kUnits;
-              ok = mbar_wait(&B->lat_empty[s], ((u / C::kUnits) & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY);
+            full = &B->full[j & 3];
+            const int32_t x_rope = Q8 ? 0 : kLatent;
+            if (g > 0) tma_prefetch_l2_2d(&p.tm_kv, x_rope, y);
+            for (int h = 0; h < 2 && ok && !Q8; ++h) {
+              ok = free_unit(h);
               if (!ok) break;
-              mbar_arrive_expect_tx(&B->lat_full[s], kUnit);
-              for (int b = 0; b < 4; ++b)
-                tma_load_2d(smem + s * kUnit + b * kBox, &p.tm_kv, &B->lat_full[s], 64 * (4 * h + b), y);
+              if (h == 0) mbar_arrive_expect_tx(full, 2 * kUnit);
+              for (int b = 4 * h; b < 4 * h + 4; ++b)
+                tma_load_2d(smem + ((2 * j + h) % C::kUnits) * kUnit + (b & 3) * kBox, &p.tm_kv, full, 64 * b, y);
             }
+            if (ok && g > 0) ok = mbar_wait(&B->s_full, (g - 1) & 1, abort, p.err, ERR_TIMEOUT_EMPTY);
             if (!ok) break;
-            ok = mbar_wait(&B->rp_empty[g & 1], ((g >> 1) & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY);
-            if (!ok) break;
-            mbar_arrive_expect_tx(&B->rp_full[g & 1], kBox);
-            tma_load_2d(smem + C::OFF_RP + (g & 1) * kBox, &p.tm_kv, &B->rp_full[g & 1], Q8 ? 0 : kLatent, y);
-            rp = g + 1;
+            mbar_arrive_expect_tx(&B->rope_full, kBox);
+            tma_load_2d(smem + C::OFF_R, &p.tm_kv, &B->rope_full, x_rope, y);
           }
         }
-        if (!ok) {  // copies in flight land before the CTA exits
-          for (uint32_t k = u > C::kUnits ? u - C::kUnits : 0; !Q8 && k < u; ++k)
-            drain_wait(&B->lat_full[k % C::kUnits], (k / C::kUnits) & 1, p.err);
-          for (uint32_t k = rp > 2 ? rp - 2 : 0; k < rp; ++k) drain_wait(&B->rp_full[k & 1], (k >> 1) & 1, p.err);
-          if (Q8) {  // query units: no barrier phase is left to wait on for sure, so wait long enough
-            const uint64_t t0 = globaltimer();
-            while (globaltimer() - t0 < 1000000ull) {
-            }
+        if (!ok) {  // copies in flight land before the CTA exits; no barrier tells of a half-issued step
+          const uint64_t from = globaltimer();
+          while (globaltimer() - from < 1000000ull) {
           }
         }
       }
     } else if (warp == 1 && fit) {
       if (elect_one()) {
         constexpr uint32_t id_qk = idesc_f16(1, 1, 0, 0, kTreeRows, kTreeKeys);  // both K-major
-        constexpr uint32_t id_pv = idesc_f16(1, 1, 0, 1, kTreeRows, 256);        // V rows as they lie: MN-major
-        const uint32_t k_lo = desc_lo(s_base, 16), v_lo = desc_lo(s_base, kBox);  // K-major boxes; MN-major, 64 dims a box
-        constexpr uint32_t kU16 = kUnit / 16, kB16 = kBox / 16;
-        uint32_t g = 0, u = 0;
+        const uint32_t k_lo = desc_lo(s_base, 16);
+        uint32_t g = 0, j = 0;
         bool ok = true;
-        // the tile whose P.V has not been issued yet
-        bool pend = false, pend_first = false;
-        uint32_t pend_u = 0;
-        int pend_n = 0;
-        auto pv = [&]() -> bool {  // O += P . V of tile g - 1
-          const uint32_t r = (g - 1) & 1;
-          if (!mbar_wait(&B->p_full, r, abort, p.err, ERR_TIMEOUT_FULL)) return false;
-          if (pend_first && pend_n > 0 && !mbar_wait(&B->o_empty, (pend_n - 1) & 1, abort, p.err, ERR_TIMEOUT_EMPTY))
-            return false;
+        int n0 = p.items[it0].tile0, n1 = p.items[it0].tile1;  // read one item ahead
+        for (int it = it0, n = 0; it < it1 && ok; ++it, ++n) {
+          const int t0 = n0, t1 = n1;
+          if (it + 1 < it1) {
+            n0 = p.items[it + 1].tile0;
+            n1 = p.items[it + 1].tile1;
+          }
+          // ---- the query's boxes to tensor memory, once the scores before have read theirs
+          if (n > 0) ok = mbar_wait(&B->q_done, (n - 1) & 1, abort, p.err, ERR_TIMEOUT_MMA);
+          if (ok) ok = mbar_wait(&B->full[j & 3], (j >> 2) & 1, abort, p.err, ERR_TIMEOUT_FULL);
+          if (!ok) break;
           tc_fence_after();
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t s = (pend_u + h) % C::kUnits;
+          for (int b = 0; b < C::kQT; ++b)
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              mma_f16_ws_ss(tmem + 128 * h, desc_of(k_lo + C::OFF_RP / 16 + r * kB16 + kk * 2),
-                            desc_of(v_lo + s * kU16 + kk * 128), id_pv, !pend_first || kk > 0);
-            mma_commit(&B->lat_empty[s]);
-          }
-          mma_commit(&B->rp_empty[r]);
-          mma_commit(&B->pv_done);
-          pend = false;
-          return true;
-        };
-        for (int it = it0, n = 0; it < it1 && ok; ++it, ++n) {
-          const int t0 = p.items[it].tile0, t1 = p.items[it].tile1;
-          // Q8: the first tile's second unit takes the place of the last tile's
-          // first one, which that tile's P.V frees
-          if (Q8 && pend) ok = pv();
-          // ---- the query's boxes to tensor memory, once the scores before have read theirs
-          if (ok && n > 0) ok = mbar_wait(&B->q_done, (n - 1) & 1, abort, p.err, ERR_TIMEOUT_MMA);
-          for (int h = 0; h < 2 && ok; ++h, ++u) {
-            const uint32_t s = u % C::kUnits;
-            ok = mbar_wait(&B->lat_full[s], (u / C::kUnits) & 1, abort, p.err, ERR_TIMEOUT_FULL);
+            for (int c = 0; c < 8; ++c)
+              tmem_cp_64x128b_x2(tmem + C::kColQ + 32 * b + 4 * c,
+                                 desc_of(k_lo + ((2 * j + (b >> 2)) % C::kUnits) * kU16 + (b & 3) * kB16 + c));
+          mma_commit(&B->done[j & 3]);
+          ++j;
+          for (int t = t0; t < t1; ++t, ++j, ++g) {
+            // ---- S = Q . K^T
+            ok = mbar_wait(&B->full[j & 3], (j >> 2) & 1, abort, p.err, ERR_TIMEOUT_FULL) &&
+                 mbar_wait(&B->s_empty, (g & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY);
+            if (ok && t == t0) ok = mbar_wait(&B->qs_full, n & 1, abort, p.err, ERR_TIMEOUT_FULL);
             if (!ok) break;
             tc_fence_after();
-#pragma unroll
-            for (int b = 0; b < (h ? C::kQT - 4 : 4); ++b)
-#pragma unroll
-              for (int c = 0; c < 8; ++c)
-                tmem_cp_64x128b_x2(tmem + C::kColQ + 32 * (4 * h + b) + 4 * c, desc_of(k_lo + s * kU16 + b * kB16 + c));
-            mma_commit(&B->lat_empty[s]);
-          }
-          for (int t = t0; t < t1 && ok; ++t, ++g, u += 2) {
-            // The scores of this tile go before the P.V of the one before, which
-            // waits for its softmax -- unless this tile is still on its way.
-            if (pend && !mbar_test(&B->lat_full[(u + 1) % C::kUnits], ((u + 1) / C::kUnits) & 1)) ok = pv();
-            // ---- S = Q . K^T
-            if (ok) ok = mbar_wait(&B->s_empty, (g & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY);
             const uint32_t s_lat = tmem + C::kColS, s_rope = s_lat + (Q8 ? 32 : 0);
             // opaque, or the compiler keeps all 36 operand addresses in registers across tiles
             uint32_t tq = tmem + C::kColQ, kl = k_lo;
             asm volatile("" : "+r"(tq), "+r"(kl));
+            bool rope_ok = false;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t s = (u + h) % C::kUnits;
-              if (ok) ok = mbar_wait(&B->lat_full[s], ((u + h) / C::kUnits) & 1, abort, p.err, ERR_TIMEOUT_FULL);
-              if (ok && h && t == t0) ok = mbar_wait(&B->qs_full, n & 1, abort, p.err, ERR_TIMEOUT_FULL);
-              if (!ok) break;
-              tc_fence_after();
+            for (int b = 0; b < 8; ++b) {
+              const uint32_t s = (2 * j + (b >> 2)) % C::kUnits;
+              if (b == 7) rope_ok = mbar_test(&B->rope_full, g & 1);  // MMAs are queued meanwhile
 #pragma unroll
-              for (int b = 0; b < 4; ++b)
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
-                  const uint64_t kd = desc_of(kl + s * kU16 + b * kB16 + kk * 2);
-                  const int qb = 4 * h + b;
-                  if (qb < C::kQT)
-                    mma_f16_ws_ts(s_lat, tq + 32 * qb + 8 * kk, kd, id_qk, qb + kk > 0);
-                  else
-                    mma_f16_ws_ss(s_lat, desc_of(kl + C::OFF_QS / 16 + (qb - C::kQT) * kB16 + kk * 2), kd, id_qk, 1u);
-                }
+              for (int kk = 0; kk < 4; ++kk) {
+                const uint64_t kd = desc_of(kl + s * kU16 + (b & 3) * kB16 + kk * 2);
+                if (b < C::kQT)
+                  mma_f16_ws_ts(s_lat, tq + 32 * b + 8 * kk, kd, id_qk, b + kk > 0);
+                else
+                  mma_f16_ws_ss(s_lat, desc_of(kl + C::OFF_QS / 16 + (b - C::kQT) * kB16 + kk * 2), kd, id_qk, 1u);
+              }
             }
-            if (ok) ok = mbar_wait(&B->rp_full[g & 1], (g >> 1) & 1, abort, p.err, ERR_TIMEOUT_FULL);
+            if (!rope_ok) ok = mbar_wait(&B->rope_full, g & 1, abort, p.err, ERR_TIMEOUT_FULL);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
               mma_f16_ws_ss(s_rope, desc_of(kl + C::OFF_QS / 16 + (8 - C::kQT) * kB16 + kk * 2),
-                            desc_of(kl + C::OFF_RP / 16 + (g & 1) * kB16 + kk * 2), id_qk, Q8 ? kk > 0 : 1u);
+                            desc_of(kl + C::OFF_R / 16 + kk * 2), id_qk, Q8 ? kk > 0 : 1u);
             mma_commit(&B->s_full);
             if (t + 1 == t1) mma_commit(&B->q_done);
-            if (pend) ok = pv();
-            pend = true;
-            pend_first = t == t0;
-            pend_u = u;
-            pend_n = n;
           }
         }
-        if (ok && pend) pv();
         // issued tensor-core work ends before tensor memory is released
-        mma_commit(&B->drain);
-        drain_wait(&B->drain, 0, p.err);
+        mma_commit(&B->drain[0]);
+        drain_wait(&B->drain[0], 0, p.err);
+      }
+    } else if (warp == 3 && fit) {
+      if (elect_one()) {
+        constexpr uint32_t id_pv = idesc_f16(1, 1, 0, 1, kTreeRows, 256);  // V rows as they lie: MN-major
+        const uint32_t p_lo = desc_lo(s_base + C::OFF_P, 16), v_lo = desc_lo(s_base, kBox);
+        uint32_t g = 0, j = 0;
+        bool ok = true;
+        int n0 = p.items[it0].tile0, n1 = p.items[it0].tile1;
+        for (int it = it0, n = 0; it < it1 && ok; ++it, ++n) {
+          const int t0 = n0, t1 = n1;
+          if (it + 1 < it1) {
+            n0 = p.items[it + 1].tile0;
+            n1 = p.items[it + 1].tile1;
+          }
+          ++j;  // the query
+          for (int t = t0; t < t1; ++t, ++j, ++g) {
+            // ---- O += P . V
+            ok = mbar_wait(&B->p_full, g & 1, abort, p.err, ERR_TIMEOUT_FULL) &&
+                 mbar_wait(&B->full[j & 3], (j >> 2) & 1, abort, p.err, ERR_TIMEOUT_FULL);
+            if (ok && t == t0 && n > 0) ok = mbar_wait(&B->o_empty, (n - 1) & 1, abort, p.err, ERR_TIMEOUT_EMPTY);
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t pl = p_lo, vl = v_lo;
+            asm volatile("" : "+r"(pl), "+r"(vl));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t s = (2 * j + h) % C::kUnits;
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk)
+                mma_f16_ws_ss(tmem + 128 * h, desc_of(pl + kk * 2), desc_of(vl + s * kU16 + kk * 128), id_pv,
+                              t > t0 || kk > 0);
+            }
+            mma_commit(&B->done[j & 3]);
+          }
+        }
+        mma_commit(&B->drain[1]);
+        drain_wait(&B->drain[1], 0, p.err);
       }
     } else if (warp == 2 && fit) {
       if (elect_one()) {
@@ -601,21 +616,26 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
       const int tid = threadIdx.x - 128;
       const int row = tid & 63, half = tid >> 6;
       const uint32_t lanes = static_cast<uint32_t>(32 * (warp - 4)) << 16;
-      uint32_t g = 0, u = 0;
+      uint32_t g = 0, j = 0;
       bool bad = false;
+      auto load_mask = [&](const TreeItem &im) -> uint64_t {
+        return row < im.nn * kHeads ? p.mask[im.node0 + row / kHeads] : 0;
+      };
+      TreeItem nx = p.items[it0];  // descriptors and masks are read one item ahead
+      uint64_t next_mask = load_mask(nx);
       for (int it = it0; it < it1 && !bad; ++it) {
-        const TreeItem im = p.items[it];
-        u += 2;  // its query
+        const TreeItem im = nx;
+        if (it + 1 < it1) nx = p.items[it + 1];
+        ++j;  // its query
         const bool real = row < im.nn * kHeads;
-        uint64_t mask = real ? p.mask[im.node0 + row / kHeads] : 0;
+        uint64_t mask = next_mask;
         if (im.tree < 64) mask &= (uint64_t(1) << im.tree) - 1;
         float m = -INFINITY, l = 0.f;
-        for (int t = im.tile0; t < im.tile1; ++t, ++g, u += 2) {
+        for (int t = im.tile0; t < im.tile1; ++t, ++g, ++j) {
           bad |= !mbar_wait(&B->s_full, g & 1, abort, p.err, ERR_TIMEOUT_MMA);
           const float *ks = B->scale[g % kScaleRing] + 32 * half;
           if (Q8)  // the converters' row scales
-            bad |= !mbar_wait(&B->lat_full[(u + 1) % C::kUnits], ((u + 1) / C::kUnits) & 1, abort, p.err,
-                              ERR_TIMEOUT_FULL);
+            bad |= !mbar_wait(&B->full[j & 3], (j >> 2) & 1, abort, p.err, ERR_TIMEOUT_FULL);
           tc_fence_after();
           float s[32];
           tmem_ld32(tmem + C::kColS + lanes, s);
@@ -655,7 +675,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
                 const uint64_t rows = static_cast<uint64_t>(B->nonfinite[0] & B->nonfinite[1]) |
                                       static_cast<uint64_t>(B->nonfinite[2] & B->nonfinite[3]) << 32;
                 const uint32_t box = tid >> 3 & 7;
-                uint8_t *v = smem + ((u + (box >> 2)) % C::kUnits) * kUnit + (box & 3) * kBox + (tid & 7) * 16;
+                uint8_t *v = smem + ((2 * j + (box >> 2)) % C::kUnits) * kUnit + (box & 3) * kBox + (tid & 7) * 16;
                 for (int k = tid >> 6; k < kTreeKeys; k += 2)
                   if (rows >> k & 1) *reinterpret_cast<uint4 *>(v + k * 128) = make_uint4(0u, 0u, 0u, 0u);
               }
@@ -680,7 +700,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
             const float mn = fmaxf(m, mx);
             const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
             if (t > im.tile0) {
-              bad |= !mbar_wait(&B->pv_done, (g - 1) & 1, abort, p.err, ERR_TIMEOUT_MMA);
+              bad |= !wait_done(B, j - 1, abort, p.err);
               tc_fence_after();
 #pragma unroll
               for (int c = 0; c < 256; c += 32) {
@@ -708,8 +728,9 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
             }
             pk[c / 2] = pack_bf16(p0, p1);
           }
-          // in the place of the tile's rope, which the scores have read
-          uint8_t *pd = smem + C::OFF_RP + (g & 1) * kBox + (row >> 3) * 1024 + (row & 7) * 128;
+          // the P before is read until its P.V is done
+          if (g > 0) bad |= !wait_done(B, t > im.tile0 ? j - 1 : j - 2, abort, p.err);
+          uint8_t *pd = smem + C::OFF_P + (row >> 3) * 1024 + (row & 7) * 128;
 #pragma unroll
           for (int c = 0; c < 4; ++c)
             *reinterpret_cast<uint4 *>(pd + ((4 * half + c) ^ (row & 7)) * 16) =
@@ -721,7 +742,8 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
         }
         if (bad) break;
         // ---- epilogue
-        bad |= !mbar_wait(&B->pv_done, (g - 1) & 1, abort, p.err, ERR_TIMEOUT_MMA);
+        next_mask = load_mask(nx);
+        bad |= !wait_done(B, j - 1, abort, p.err);
         B->red[2][tid] = l;
         if (named_bar_or(1, 128, bad)) {
           bad = true;
@@ -777,9 +799,9 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
     // the CTA's tiles in order
     int it = it0, t = it0 < it1 ? p.items[it0].tile0 : 0, t1 = it0 < it1 ? p.items[it0].tile1 : 0;
     long long row0 = it0 < it1 ? p.items[it0].row0 : 0;
-    uint32_t u = 0, u0 = 0, u1 = 0;  // units of the ring so far; of the tiles in v0 and v1
-    bool fresh = true;               // the next tile is its item's first: two query units come before it
-    auto load = [&](uint4(&v)[8], float &sc, uint32_t &un) -> bool {
+    uint32_t j = 0, j0 = 0, j1 = 0;  // steps so far; of the tiles in v0 and v1
+    bool fresh = true;               // the next tile is its item's first: the query's step comes before it
+    auto load = [&](uint4(&v)[8], float &sc, uint32_t &step) -> bool {
       if (it < it1 && t >= t1) {
         if (++it < it1) {
           t = p.items[it].tile0;
@@ -789,10 +811,9 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
         }
       }
       if (it >= it1) return false;
-      if (fresh) u += 2;
+      if (fresh) ++j;
       fresh = false;
-      un = u;
-      u += 2;
+      step = j++;
       const long long first = row0 + static_cast<long long>(kTreeKeys) * t;
       const uint4 *src = reinterpret_cast<const uint4 *>(p.lat8 + min(first + r, last) * kLatent) + c;
 #pragma unroll
@@ -802,12 +823,11 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
       return true;
     };
     uint32_t g = 0;
-    auto store = [&](const uint4(&v)[8], float sc, uint32_t un) -> bool {
+    auto store = [&](const uint4(&v)[8], float sc, uint32_t step) -> bool {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t slot = (un + h) % C::kUnits;
-        if (!mbar_wait(&B->lat_empty[slot], (((un + h) / C::kUnits) & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY))
-          return false;
+        const uint32_t u = 2 * step + h, slot = u % C::kUnits;
+        if (u >= C::kUnits && !wait_done(B, (u - C::kUnits) >> 1, abort, p.err)) return false;
         uint8_t *dst = smem + slot * kUnit + (r >> 3) * 1024 + (r & 7) * 128;
         if (h == 1 && tid < kTreeKeys) B->scale[g % kScaleRing][tid] = sc;
 #pragma unroll
@@ -818,21 +838,21 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
           *reinterpret_cast<uint4 *>(dst + b * kBox + ((2 * c + 1) ^ (r & 7)) * 16) =
               make_uint4(s8x2_to_bf16<0>(x.z), s8x2_to_bf16<1>(x.z), s8x2_to_bf16<0>(x.w), s8x2_to_bf16<1>(x.w));
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&B->lat_full[slot]);
       }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&B->full[step & 3]);
       ++g;
       return true;
     };
     uint4 v0[8], v1[8];
     float sc0 = 0.f, sc1 = 0.f;
-    bool more = load(v0, sc0, u0);
+    bool more = load(v0, sc0, j0);
     while (more) {  // the next tile's rows are in flight while this one is stored
-      const bool second = load(v1, sc1, u1);
-      if (!store(v0, sc0, u0) || !second) break;
-      more = load(v0, sc0, u0);
-      if (!store(v1, sc1, u1)) break;
+      const bool second = load(v1, sc1, j1);
+      if (!store(v0, sc0, j0) || !second) break;
+      more = load(v0, sc0, j0);
+      if (!store(v1, sc1, j1)) break;
     }
   }
 
