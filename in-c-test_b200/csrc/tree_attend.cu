@@ -319,28 +319,29 @@ constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kU16 = kUnit / 16, kB16 = kBox / 16;  // in units of a matrix descriptor
 constexpr int kScaleRing = 4;
 
+constexpr int kSoftThreads = 256;    // warps 4-11: softmax and epilogue
+constexpr int kConvertWarp = 12;     // Q8: warps 12-19 load and convert the latents
+constexpr int kConvertThreads = 256;
+template <bool Q8>
+constexpr int threads() { return 128 + kSoftThreads + (Q8 ? kConvertThreads : 0); }
+
 struct Bars {
-  // of step j: [j % 4], phase j / 4.  full: its latents are there; done: its P.V
-  // (its copy to tensor memory) is, so its place is free
-  uint64_t full[4], done[4];
+  // of step j's unit h: [h][j % 4], phase j / 4.  full: its bytes are there; done:
+  // its half of the P.V (its copy to tensor memory) is, so its place is free
+  uint64_t full[2][4], done[2][4];
   uint64_t rope_full;
   uint64_t qs_full, q_done;  // q_done: the item's last scores are done
   uint64_t s_full, s_empty;
   uint64_t p_full, o_empty, drain[2];
   uint32_t tmem_base;
   int abort;
-  uint32_t nonfinite[4];
-  float red[3][128];  // row maxima of alternate tiles; row sums at an item's end
-  float scale[kScaleRing][kTreeKeys];  // Q8: row scales of the tiles in flight
+  uint32_t nonfinite[8];
+  float red[2][kSoftThreads];  // row maxima, row sums: alternate exchanges
 };
+typedef float Scales[kScaleRing][kTreeKeys];  // Q8, behind Bars: row scales of the tiles in flight
 template <bool Q8>
-constexpr uint32_t smem_bytes() { return Cfg<Q8>::OFF_BAR + sizeof(Bars); }
+constexpr uint32_t smem_bytes() { return Cfg<Q8>::OFF_BAR + sizeof(Bars) + (Q8 ? sizeof(Scales) : 0); }
 static_assert(smem_bytes<false>() <= 232448 && smem_bytes<true>() <= 232448, "shared memory budget");
-
-constexpr int kConvertWarp = 8;  // Q8: warps 8-15 load and convert the latents
-constexpr int kConvertThreads = 256;
-template <bool Q8>
-constexpr int threads() { return Q8 ? 256 + kConvertThreads : 256; }
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -358,26 +359,64 @@ __device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo_bytes) 
   return saddr >> 4 | (lbo_bytes >> 4) << 16;
 }
 
-// Two of the four int8 in `w` (bytes i, i + 1) as bf16.  0x4300 is 128 with a
-// unit in the last place: 128 + (b & 127) less 128, or 256 for a negative b
-// (128 + 128 = 0x4380), is b exactly.
-template <int I>
-__device__ __forceinline__ uint32_t s8x2_to_bf16(uint32_t w) {
-  const uint32_t v = __byte_perm(w, 0u, I == 0 ? 0x4140 : 0x4342);
-  const uint32_t lo = (v & 0x007f007fu) | 0x43004300u, hi = (v & 0x00800080u) | 0x43004300u;
-  const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&lo),
-                                   *reinterpret_cast<const __nv_bfloat162 *>(&hi));
-  return *reinterpret_cast<const uint32_t *>(&d);
+// Sixteen bf16, in one store where they are aligned to 32 bytes.
+__device__ __forceinline__ void store_bf16x16(uint16_t *dst, bool aligned, const float (&o)[16]) {
+  uint32_t v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = pack_bf16(o[2 * i], o[2 * i + 1]);
+  if (aligned) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4 *>(dst)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<uint4 *>(dst)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+  }
+}
+
+// 32 bytes in one load where they are aligned to it.
+__device__ __forceinline__ void load_32(const int8_t *src, bool aligned, uint4 &a, uint4 &b) {
+  if (!aligned) {
+    a = __ldg(reinterpret_cast<const uint4 *>(src));
+    b = __ldg(reinterpret_cast<const uint4 *>(src) + 1);
+    return;
+  }
+  asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+      : "l"(src));
+}
+
+// Four int8 b as bf16, exactly, from u = b + 128 in 0..255 (flip_signs).  The bf16
+// 0x4300 + u is f = 128 + u for u < 128 and 256 + 2 (u - 128) above, so f - 256
+// is b, or 2 b where b > 0; relu(f / 2 - 128) is what is too much.  Three
+// operations of a pair go to the fp16 pipe and 1.5 to the integer pipe, which is
+// half as fast and bound a form with masks (4 x 32768 rows 10 % slower).
+__device__ __forceinline__ void flip_signs(uint32_t &w) { asm volatile("xor.b32 %0, %0, 0x80808080;" : "+r"(w)); }
+__device__ __forceinline__ uint2 u8x4_to_bf16(uint32_t u) {
+  const uint32_t f[2] = {__byte_perm(u, 0x43434343u, 0x5140), __byte_perm(u, 0x43434343u, 0x5342)};
+  uint32_t x[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162 *>(&f[i]);
+    const __nv_bfloat162 over = __hfma2_relu(v, __floats2bfloat162_rn(0.5f, 0.5f), __floats2bfloat162_rn(-128.f, -128.f));
+    const __nv_bfloat162 d = __hsub2(__hsub2(v, __floats2bfloat162_rn(256.f, 256.f)), over);
+    x[i] = *reinterpret_cast<const uint32_t *>(&d);
+  }
+  return make_uint2(x[0], x[1]);
 }
 
 }  // namespace treek
 
 using namespace treek;
 
-// Waits until step `k` is done.  Steps share four barriers, so nobody may ask
-// for a step that is four or more behind the last one loaded.
-__device__ __forceinline__ bool wait_done(Bars *B, uint32_t k, volatile int *abort, uint32_t *err) {
-  return mbar_wait(&B->done[k & 3], (k >> 2) & 1, abort, err, ERR_TIMEOUT_EMPTY);
+// Waits until unit u = 2 step + half is done (or full).  Steps share four
+// barriers, so nobody may ask for a step that is four or more behind the last
+// one loaded.
+__device__ __forceinline__ bool wait_done(Bars *B, uint32_t u, volatile int *abort, uint32_t *err) {
+  return mbar_wait(&B->done[u & 1][(u >> 1) & 3], (u >> 3) & 1, abort, err, ERR_TIMEOUT_EMPTY);
+}
+__device__ __forceinline__ bool wait_full(Bars *B, uint32_t u, volatile int *abort, uint32_t *err) {
+  return mbar_wait(&B->full[u & 1][(u >> 1) & 3], (u >> 3) & 1, abort, err, ERR_TIMEOUT_FULL);
 }
 
 // One CTA per SM, roles by warp:
@@ -386,9 +425,11 @@ __device__ __forceinline__ bool wait_done(Bars *B, uint32_t k, volatile int *abo
 //          until the MMAs before it have left the queue, so one thread for both
 //          leaves the tensor core idle 500 of a tile's 2150 cycles
 //   2      loader of the query boxes that stay in shared memory
-//   4-7    softmax and epilogue: thread t has query row t % 64 and keys
-//          32 (t / 64) .. + 31 of a tile (where .ws puts them)
-//   8-15   Q8: latents from global memory, as bf16 into the ring
+//   4-11   softmax and epilogue: thread t has query row t % 64 and, of a tile's
+//          keys, 32 (t / 64 % 2) + 16 (t / 128) .. + 15 (.ws puts keys 32 and up
+//          into lanes 64-127); of O, the columns 128 (t / 128) .. + 127.  Four
+//          warps took 2500 cycles a Q8 tile and were what bounded it.
+//   12-19  Q8: latents from global memory, as bf16 into the ring
 //
 // The latent ring runs in steps of two units, half a tile each.  An item is a
 // step of query boxes, which the issuer copies to tensor memory (tcgen05.cp),
@@ -399,24 +440,27 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
   using C = Cfg<Q8>;
   extern __shared__ __align__(1024) uint8_t smem[];
   Bars *B = reinterpret_cast<Bars *>(smem + C::OFF_BAR);
+  Scales &scales = *reinterpret_cast<Scales *>(smem + C::OFF_BAR + sizeof(Bars));
   const uint32_t s_base = smem_u32(smem);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int it0 = p.cta_item[blockIdx.x], it1 = p.cta_item[blockIdx.x + 1];
+  const int it0 = p.cta_item[blockIdx.x];
+  int it1 = p.cta_item[blockIdx.x + 1];
   volatile int *abort = &B->abort;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(&B->full[i], Q8 ? kConvertThreads / 32 : 1);
-      mbar_init(&B->done[i], 1);
-    }
+    for (int h = 0; h < 2; ++h)
+      for (int i = 0; i < 4; ++i) {
+        mbar_init(&B->full[h][i], Q8 ? kConvertThreads / 32 : 1);
+        mbar_init(&B->done[h][i], 1);
+      }
     mbar_init(&B->rope_full, 1);
     mbar_init(&B->qs_full, 1);
     mbar_init(&B->q_done, 1);
     mbar_init(&B->s_full, 1);
-    mbar_init(&B->s_empty, 4);
-    mbar_init(&B->p_full, 4);
-    mbar_init(&B->o_empty, 4);
+    mbar_init(&B->s_empty, kSoftThreads / 32);
+    mbar_init(&B->p_full, kSoftThreads / 32);
+    mbar_init(&B->o_empty, kSoftThreads / 32);
     mbar_init(&B->drain[0], 1);
     mbar_init(&B->drain[1], 1);
     B->abort = 0;
@@ -437,9 +481,8 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
   const bool fit = !*abort;  // the same for all threads
   asm volatile("griddepcontrol.launch_dependents;");
 
-  // Q8: 512 threads start with 128 registers each; 96 + 160 + 2 x 128 = 4 x 128
+  // Q8: 640 threads start with 96 registers each; 96 + 2 x 80 + 2 x 112 = 5 x 96
   if (warp < 4) {
-    if (Q8) asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     if (warp == 0 && fit) {
       if (elect_one()) {
         tma_prefetch_desc(&p.tm_q);
@@ -449,34 +492,34 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
         // the places of step j: their last steps must be done
         auto free_unit = [&](int h) -> bool {
           const uint32_t u = 2 * j + h;
-          return u < C::kUnits || wait_done(B, (u - C::kUnits) >> 1, abort, p.err);
+          return u < C::kUnits || wait_done(B, u - C::kUnits, abort, p.err);
         };
         TreeItem nx = p.items[it0];  // descriptors are read one item ahead
         for (int it = it0; it < it1 && ok; ++it) {
           const TreeItem im = nx;
           if (it + 1 < it1) nx = p.items[it + 1];
-          uint64_t *full = &B->full[j & 3];
           for (int h = 0; h < 2 && ok; ++h) {
             ok = free_unit(h);
             if (!ok) break;
-            if (h == 0) mbar_arrive_expect_tx(full, C::kQT * kBox);
+            uint64_t *full = &B->full[h][j & 3];
+            mbar_arrive_expect_tx(full, (h ? C::kQT - 4 : 4) * kBox);
             for (int b = 4 * h; b < (h ? C::kQT : 4); ++b)
               tma_load_2d(smem + ((2 * j + h) % C::kUnits) * kUnit + (b & 3) * kBox, &p.tm_q, full, 64 * b,
                           im.node0 * kHeads);
+            if (Q8)  // the barrier counts the converter warps
+              for (int i = 1; i < kConvertThreads / 32; ++i) mbar_arrive(full);
           }
           if (!ok) break;
-          if (Q8)  // the barrier counts the converter warps too
-            for (int i = 1; i < kConvertThreads / 32; ++i) mbar_arrive(full);
           ++j;
           for (int t = im.tile0; t < im.tile1 && ok; ++t, ++g, ++j) {
             const int32_t y = static_cast<int32_t>(im.row0 + static_cast<long long>(kTreeKeys) * t);
-            full = &B->full[j & 3];
             const int32_t x_rope = Q8 ? 0 : kLatent;
             if (g > 0) tma_prefetch_l2_2d(&p.tm_kv, x_rope, y);
             for (int h = 0; h < 2 && ok && !Q8; ++h) {
               ok = free_unit(h);
               if (!ok) break;
-              if (h == 0) mbar_arrive_expect_tx(full, 2 * kUnit);
+              uint64_t *full = &B->full[h][j & 3];
+              mbar_arrive_expect_tx(full, kUnit);
               for (int b = 4 * h; b < 4 * h + 4; ++b)
                 tma_load_2d(smem + ((2 * j + h) % C::kUnits) * kUnit + (b & 3) * kBox, &p.tm_kv, full, 64 * b, y);
             }
@@ -507,7 +550,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
           }
           // ---- the query's boxes to tensor memory, once the scores before have read theirs
           if (n > 0) ok = mbar_wait(&B->q_done, (n - 1) & 1, abort, p.err, ERR_TIMEOUT_MMA);
-          if (ok) ok = mbar_wait(&B->full[j & 3], (j >> 2) & 1, abort, p.err, ERR_TIMEOUT_FULL);
+          if (ok) ok = wait_full(B, 2 * j, abort, p.err) && wait_full(B, 2 * j + 1, abort, p.err);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
@@ -516,11 +559,12 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
             for (int c = 0; c < 8; ++c)
               tmem_cp_64x128b_x2(tmem + C::kColQ + 32 * b + 4 * c,
                                  desc_of(k_lo + ((2 * j + (b >> 2)) % C::kUnits) * kU16 + (b & 3) * kB16 + c));
-          mma_commit(&B->done[j & 3]);
+          mma_commit(&B->done[0][j & 3]);
+          mma_commit(&B->done[1][j & 3]);
           ++j;
           for (int t = t0; t < t1; ++t, ++j, ++g) {
             // ---- S = Q . K^T
-            ok = mbar_wait(&B->full[j & 3], (j >> 2) & 1, abort, p.err, ERR_TIMEOUT_FULL) &&
+            ok = wait_full(B, 2 * j, abort, p.err) &&
                  mbar_wait(&B->s_empty, (g & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY);
             if (ok && t == t0) ok = mbar_wait(&B->qs_full, n & 1, abort, p.err, ERR_TIMEOUT_FULL);
             if (!ok) break;
@@ -529,11 +573,17 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
             // opaque, or the compiler keeps all 36 operand addresses in registers across tiles
             uint32_t tq = tmem + C::kColQ, kl = k_lo;
             asm volatile("" : "+r"(tq), "+r"(kl));
-            bool rope_ok = false;
+            bool hi_ok = false, rope_ok = false;
 #pragma unroll
             for (int b = 0; b < 8; ++b) {
               const uint32_t s = (2 * j + (b >> 2)) % C::kUnits;
-              if (b == 7) rope_ok = mbar_test(&B->rope_full, g & 1);  // MMAs are queued meanwhile
+              if (b == 3) hi_ok = mbar_test(&B->full[1][j & 3], (j >> 2) & 1);  // MMAs are queued meanwhile
+              if (b == 4) {
+                if (!hi_ok) ok = wait_full(B, 2 * j + 1, abort, p.err);
+                if (!ok) break;
+                tc_fence_after();
+              }
+              if (b == 7) rope_ok = mbar_test(&B->rope_full, g & 1);
 #pragma unroll
               for (int kk = 0; kk < 4; ++kk) {
                 const uint64_t kd = desc_of(kl + s * kU16 + (b & 3) * kB16 + kk * 2);
@@ -543,7 +593,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
                   mma_f16_ws_ss(s_lat, desc_of(kl + C::OFF_QS / 16 + (b - C::kQT) * kB16 + kk * 2), kd, id_qk, 1u);
               }
             }
-            if (!rope_ok) ok = mbar_wait(&B->rope_full, g & 1, abort, p.err, ERR_TIMEOUT_FULL);
+            if (ok && !rope_ok) ok = mbar_wait(&B->rope_full, g & 1, abort, p.err, ERR_TIMEOUT_FULL);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
@@ -574,9 +624,10 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
           ++j;  // the query
           for (int t = t0; t < t1; ++t, ++j, ++g) {
             // ---- O += P . V
-            ok = mbar_wait(&B->p_full, g & 1, abort, p.err, ERR_TIMEOUT_FULL) &&
-                 mbar_wait(&B->full[j & 3], (j >> 2) & 1, abort, p.err, ERR_TIMEOUT_FULL);
-            if (ok && t == t0 && n > 0) ok = mbar_wait(&B->o_empty, (n - 1) & 1, abort, p.err, ERR_TIMEOUT_EMPTY);
+            if (t == t0 && n > 0) ok = mbar_wait(&B->o_empty, (n - 1) & 1, abort, p.err, ERR_TIMEOUT_EMPTY);
+            if (ok)
+              ok = wait_full(B, 2 * j, abort, p.err) && wait_full(B, 2 * j + 1, abort, p.err) &&
+                   mbar_wait(&B->p_full, g & 1, abort, p.err, ERR_TIMEOUT_FULL);
             if (!ok) break;
             tc_fence_after();
             uint32_t pl = p_lo, vl = v_lo;
@@ -588,8 +639,8 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
               for (int kk = 0; kk < 4; ++kk)
                 mma_f16_ws_ss(tmem + 128 * h, desc_of(pl + kk * 2), desc_of(vl + s * kU16 + kk * 128), id_pv,
                               t > t0 || kk > 0);
+              mma_commit(&B->done[h][j & 3]);
             }
-            mma_commit(&B->done[j & 3]);
           }
         }
         mma_commit(&B->drain[1]);
@@ -610,14 +661,24 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
         if (!ok) drain_wait(&B->qs_full, (n - 1) & 1, p.err);
       }
     }
-  } else if (warp < 8) {
-    if (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+  } else if (warp < kConvertWarp) {
+    if (Q8) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     if (fit) {
       const int tid = threadIdx.x - 128;
-      const int row = tid & 63, half = tid >> 6;
-      const uint32_t lanes = static_cast<uint32_t>(32 * (warp - 4)) << 16;
+      const int row = tid & 63, half = tid >> 6 & 1, part = tid >> 7;
+      const int key0 = 32 * half + 16 * part;  // the thread's first key of a tile
+      const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
       uint32_t g = 0, j = 0;
       bool bad = false;
+      uint32_t x = 0;  // exchanges so far
+      // the four values of a row, in the same order for all of its threads
+      auto exchange = [&](float v, float(&r)[4]) {
+        B->red[x & 1][tid] = v;
+        bad = named_bar_or(1, kSoftThreads, bad);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = B->red[x & 1][row + 64 * i];
+        ++x;
+      };
       auto load_mask = [&](const TreeItem &im) -> uint64_t {
         return row < im.nn * kHeads ? p.mask[im.node0 + row / kHeads] : 0;
       };
@@ -630,36 +691,32 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
         const bool real = row < im.nn * kHeads;
         uint64_t mask = next_mask;
         if (im.tree < 64) mask &= (uint64_t(1) << im.tree) - 1;
-        float m = -INFINITY, l = 0.f;
+        float m = -INFINITY, l = 0.f, r[4];
         for (int t = im.tile0; t < im.tile1; ++t, ++g, ++j) {
           bad |= !mbar_wait(&B->s_full, g & 1, abort, p.err, ERR_TIMEOUT_MMA);
-          const float *ks = B->scale[g % kScaleRing] + 32 * half;
-          if (Q8)  // the converters' row scales
-            bad |= !mbar_wait(&B->full[j & 3], (j >> 2) & 1, abort, p.err, ERR_TIMEOUT_FULL);
           tc_fence_after();
-          float s[32];
-          tmem_ld32(tmem + C::kColS + lanes, s);
-          tmem_wait_ld();
+          float s[16];
+          tmem_ld16(tmem + C::kColS + 16 * part + lanes, s);
+          const float *ks = scales[g % kScaleRing] + key0;
           if (Q8) {
+            float sr[16];
+            tmem_ld16(tmem + C::kColS + 32 + 16 * part + lanes, sr);
+            bad |= !wait_full(B, 2 * j + 1, abort, p.err);  // the converters' row scales
+            tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; i += 16) {
-              float sr[16];
-              tmem_ld16(tmem + C::kColS + 32 + i + lanes, sr);
-              tmem_wait_ld();
-#pragma unroll
-              for (int c = 0; c < 16; ++c) s[i + c] = fmaf(s[i + c], ks[i + c], sr[c]);
-            }
+            for (int c = 0; c < 16; ++c) s[c] = fmaf(s[c], ks[c], sr[c]);
+          } else {
+            tmem_wait_ld();
           }
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&B->s_empty);
-          const int k0 = kTreeKeys * t + 32 * half;  // the thread's first key
-          uint32_t seen = 0xffffffffu;
           const bool masked = kTreeKeys * (t + 1) > im.len;
+          uint32_t seen = 0xffffu;
           if (masked) {
-            const int d = k0 - im.len;  // drafted row of the first key
+            const int d = kTreeKeys * t + key0 - im.len;  // drafted row of the first key
             seen = d >= 0 ? (d < 64 ? static_cast<uint32_t>(mask >> d) : 0u)
-                          : (d > -32 ? static_cast<uint32_t>(mask << -d) | (0xffffffffu >> (32 + d)) : 0xffffffffu);
+                          : (d > -16 ? static_cast<uint32_t>(mask << -d) | (0xffffu >> (16 + d)) : 0xffffu);
             if (!Q8) {
               // A hidden row gets p = 0, but 0 times an infinity or a NaN of the
               // row itself is NaN in the P.V product.  Such a row gives a score
@@ -667,49 +724,49 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
               // does so with every row, but only its own): clear those rows.
               uint32_t nf = 0;
 #pragma unroll
-              for (int c = 0; c < 32; ++c) nf |= ((__float_as_uint(s[c]) & 0x7f800000u) == 0x7f800000u) ? 1u << c : 0u;
-              if (named_bar_or(2, 128, (nf & ~seen) != 0)) {
+              for (int c = 0; c < 16; ++c) nf |= ((__float_as_uint(s[c]) & 0x7f800000u) == 0x7f800000u) ? 1u << c : 0u;
+              if (named_bar_or(2, kSoftThreads, (nf & ~seen) != 0)) {
                 const uint32_t all = __reduce_and_sync(0xffffffffu, nf);
                 if (lane == 0) B->nonfinite[warp - 4] = all;
-                named_bar_sync(2, 128);
-                const uint64_t rows = static_cast<uint64_t>(B->nonfinite[0] & B->nonfinite[1]) |
-                                      static_cast<uint64_t>(B->nonfinite[2] & B->nonfinite[3]) << 32;
+                named_bar_sync(2, kSoftThreads);
+                uint64_t rows = 0;
+                for (int i = 0; i < 4; ++i)  // half i % 2, part i / 2
+                  rows |= static_cast<uint64_t>(B->nonfinite[2 * i] & B->nonfinite[2 * i + 1])
+                          << (32 * (i & 1) + 16 * (i >> 1));
                 const uint32_t box = tid >> 3 & 7;
                 uint8_t *v = smem + ((2 * j + (box >> 2)) % C::kUnits) * kUnit + (box & 3) * kBox + (tid & 7) * 16;
-                for (int k = tid >> 6; k < kTreeKeys; k += 2)
+                for (int k = tid >> 6; k < kTreeKeys; k += 4)
                   if (rows >> k & 1) *reinterpret_cast<uint4 *>(v + k * 128) = make_uint4(0u, 0u, 0u, 0u);
               }
             }
           }
           float mx = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            s[c] = (seen >> c & 1) ? s[c] * p.scale_log2 : -INFINITY;
-            mx = fmaxf(mx, s[c]);
-          }
-          // the other half of the row's keys
-          B->red[g & 1][tid] = mx;
-          if (named_bar_or(1, 128, bad)) {
-            bad = true;
-            break;
-          }
-          mx = fmaxf(mx, B->red[g & 1][tid ^ 64]);
-          // The reference maximum moves only when a score exceeds it by 2^8; both
-          // warps of a row decide alike.
+          for (int c = 0; c < 16; ++c) s[c] *= p.scale_log2;
+          if (masked)
+#pragma unroll
+            for (int c = 0; c < 16; ++c) s[c] = (seen >> c & 1) ? s[c] : -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 16; ++c) mx = fmaxf(mx, s[c]);
+          exchange(mx, r);
+          if (bad) break;
+          mx = fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
+          // The reference maximum moves only when a score exceeds it by 2^8; the
+          // four warps of a row decide alike.
           if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
             const float mn = fmaxf(m, mx);
             const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
             if (t > im.tile0) {
-              bad |= !wait_done(B, j - 1, abort, p.err);
+              bad |= !wait_done(B, 2 * (j - 1) + 1, abort, p.err);
               tc_fence_after();
 #pragma unroll
-              for (int c = 0; c < 256; c += 32) {
-                float o[32];
-                tmem_ld32(tmem + c + lanes, o);
+              for (int c = 0; c < 128; c += 16) {
+                float o[16];
+                tmem_ld16(tmem + 128 * part + c + lanes, o);
                 tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] *= alpha;
-                tmem_st32(tmem + c + lanes, o);
+                for (int i = 0; i < 16; ++i) o[i] *= alpha;
+                tmem_st16(tmem + 128 * part + c + lanes, o);
               }
               tmem_wait_st();
             }
@@ -717,24 +774,26 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
             m = mn;
           }
           const float ref = m == -INFINITY ? 0.f : m;  // a row that has seen nothing: exp2(-inf) = 0
-          uint32_t pk[16];
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            float p0 = ex2(s[c] - ref), p1 = ex2(s[c + 1] - ref);
-            l += p0 + p1;
-            if (Q8) {  // O accumulates p * scale * int8 row; a hidden row's scale may be anything
-              p0 = (seen >> c & 1) ? p0 * ks[c] : 0.f;
-              p1 = (seen >> (c + 1) & 1) ? p1 * ks[c + 1] : 0.f;
-            }
-            pk[c / 2] = pack_bf16(p0, p1);
+          for (int c = 0; c < 16; ++c) {
+            s[c] = ex2(s[c] - ref);
+            l += s[c];
+          }
+          if (Q8) {  // O accumulates p * scale * int8 row
+#pragma unroll
+            for (int c = 0; c < 16; ++c) s[c] *= ks[c];
+            if (masked)  // a hidden row's scale may be anything
+#pragma unroll
+              for (int c = 0; c < 16; ++c) s[c] = (seen >> c & 1) ? s[c] : 0.f;
           }
           // the P before is read until its P.V is done
-          if (g > 0) bad |= !wait_done(B, t > im.tile0 ? j - 1 : j - 2, abort, p.err);
+          if (g > 0) bad |= !wait_done(B, 2 * (t > im.tile0 ? j - 1 : j - 2) + 1, abort, p.err);
           uint8_t *pd = smem + C::OFF_P + (row >> 3) * 1024 + (row & 7) * 128;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<uint4 *>(pd + ((4 * half + c) ^ (row & 7)) * 16) =
-                make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+          for (int c = 0; c < 2; ++c)
+            *reinterpret_cast<uint4 *>(pd + ((key0 / 8 + c) ^ (row & 7)) * 16) =
+                make_uint4(pack_bf16(s[8 * c], s[8 * c + 1]), pack_bf16(s[8 * c + 2], s[8 * c + 3]),
+                           pack_bf16(s[8 * c + 4], s[8 * c + 5]), pack_bf16(s[8 * c + 6], s[8 * c + 7]));
           fence_proxy_async_smem();
           tc_fence_before();
           __syncwarp();
@@ -743,45 +802,38 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
         if (bad) break;
         // ---- epilogue
         next_mask = load_mask(nx);
-        bad |= !wait_done(B, j - 1, abort, p.err);
-        B->red[2][tid] = l;
-        if (named_bar_or(1, 128, bad)) {
-          bad = true;
-          break;
-        }
+        bad |= !wait_done(B, 2 * (j - 1) + 1, abort, p.err);
+        exchange(l, r);
+        if (bad) break;
         tc_fence_after();
-        l += B->red[2][tid ^ 64];
+        l = (r[0] + r[1]) + (r[2] + r[3]);
         const float inv = l == 0.f ? 0.f : 1.0f / l;  // nothing seen: out = 0, lse = -inf
-        if (real && half == 0) {
+        if (real && tid < kTreeRows) {
           const float lse = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
           if (im.slot >= 0)
             p.part_lse[static_cast<size_t>(im.slot) * kTreeRows + row] = lse;
           else if (p.lse)
             p.lse[static_cast<size_t>(im.node0) * kHeads + row] = lse;
         }
-        // A partial keeps the threads' own layout, [64 column quads][128 threads]
+        // A partial keeps the threads' own layout, [64 column quads][128 lanes]
         // float4: every store of a warp is 512 contiguous bytes.  (Row by row,
         // 16 bytes of 32 different rows a store, an item's end took 13000 cycles.)
-        float4 *part = reinterpret_cast<float4 *>(p.part_o) + (static_cast<size_t>(max(im.slot, 0)) * 64) * 128 + tid;
-        uint16_t *orow = p.out + (static_cast<size_t>(im.node0) * kHeads + row) * kLatent + half * 128;
+        float4 *po = reinterpret_cast<float4 *>(p.part_o) +
+                     (static_cast<size_t>(max(im.slot, 0)) * 64 + 32 * part) * 128 + (tid & 127);
+        uint16_t *orow = p.out + (static_cast<size_t>(im.node0) * kHeads + row) * kLatent + 256 * part + 128 * half;
 #pragma unroll
-        for (int c = 0; c < 256; c += 32) {
-          float o[32];
-          tmem_ld32(tmem + c + lanes, o);
+        for (int c = 0; c < 128; c += 16) {
+          float o[16];
+          tmem_ld16(tmem + 128 * part + c + lanes, o);
           tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] *= inv;
           if (im.slot >= 0) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              part[(c / 4 + i) * 128] =
-                  make_float4(o[4 * i] * inv, o[4 * i + 1] * inv, o[4 * i + 2] * inv, o[4 * i + 3] * inv);
-          } else if (real) {
-            uint4 *dst = reinterpret_cast<uint4 *>(orow + (c >> 7) * 256 + (c & 127));
-#pragma unroll
             for (int i = 0; i < 4; ++i)
-              dst[i] = make_uint4(pack_bf16(o[8 * i] * inv, o[8 * i + 1] * inv),
-                                  pack_bf16(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
-                                  pack_bf16(o[8 * i + 4] * inv, o[8 * i + 5] * inv),
-                                  pack_bf16(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+              po[(c / 4 + i) * 128] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          } else if (real) {
+            store_bf16x16(orow + c, p.out_32, o);
           }
         }
         tc_fence_before();
@@ -789,71 +841,86 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
         if (lane == 0) mbar_arrive(&B->o_empty);
       }
     }
-  } else if (Q8 && fit) {
-    // Thread t has the 16 latents c = t % 4 of row t / 4 in each of the eight
-    // boxes: four threads read 64 consecutive bytes, and the eight lanes of a
-    // store phase (two rows) fill the eight 16-byte banks of the swizzle.
+  } else if (Q8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+    if (!fit) it1 = it0;
+    // A thread loads 32 latents of a row at a time, four times a tile.  A warp
+    // covers 4 rows x 256 dims, eight whole lines: lane bits 3-4 are the box of
+    // 64 dims, bits 1-2 the row, bit 0 the half of the box, so that the eight
+    // lanes of a store phase fill the eight 16-byte banks of the swizzle.
     const int tid = threadIdx.x - 32 * kConvertWarp;
-    const int r = tid >> 2, c = tid & 3;
+    const int box = lane >> 3, r = 4 * (tid >> 5) + (lane >> 1 & 3), half = lane & 1;
     const long long last = p.rows - 1;
+    const bool aligned = (reinterpret_cast<uintptr_t>(p.lat8) & 31) == 0;
     // the CTA's tiles in order
-    int it = it0, t = it0 < it1 ? p.items[it0].tile0 : 0, t1 = it0 < it1 ? p.items[it0].tile1 : 0;
-    long long row0 = it0 < it1 ? p.items[it0].row0 : 0;
+    int it = it0, t = p.items[it0].tile0, t1 = p.items[it0].tile1;
+    long long row0 = p.items[it0].row0;
     uint32_t j = 0, j0 = 0, j1 = 0;  // steps so far; of the tiles in v0 and v1
     bool fresh = true;               // the next tile is its item's first: the query's step comes before it
+    // v: [unit][rows r and r + 32]
     auto load = [&](uint4(&v)[8], float &sc, uint32_t &step) -> bool {
-      if (it < it1 && t >= t1) {
-        if (++it < it1) {
-          t = p.items[it].tile0;
-          t1 = p.items[it].tile1;
-          row0 = p.items[it].row0;
-          fresh = true;
-        }
+      if (t >= t1 && ++it < it1) {
+        t = p.items[it].tile0;
+        t1 = p.items[it].tile1;
+        row0 = p.items[it].row0;
+        fresh = true;
       }
       if (it >= it1) return false;
       if (fresh) ++j;
       fresh = false;
       step = j++;
       const long long first = row0 + static_cast<long long>(kTreeKeys) * t;
-      const uint4 *src = reinterpret_cast<const uint4 *>(p.lat8 + min(first + r, last) * kLatent) + c;
-#pragma unroll
-      for (int b = 0; b < 8; ++b) v[b] = __ldg(src + 4 * b);
       if (tid < kTreeKeys) sc = __ldg(p.lscale + min(first + tid, last));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        load_32(p.lat8 + min(first + r + 32 * (i & 1), last) * kLatent + (4 * (i >> 1) + box) * 64 + half * 32,
+                aligned, v[2 * i], v[2 * i + 1]);
       ++t;
       return true;
     };
     uint32_t g = 0;
-    auto store = [&](const uint4(&v)[8], float sc, uint32_t step) -> bool {
+    // Stores the tile in v and loads the next one into w; false at the end.  The
+    // next loads are issued only once v has arrived (the sign flips touch all of
+    // it): loads in flight share a scoreboard, and waiting for v with w's behind
+    // it waited for w too, 1100 of 3400 cycles a tile.
+    auto turn = [&](uint4(&v)[8], float sc, uint32_t step, uint4(&w)[8], float &next_sc, uint32_t &next_step) -> bool {
+      bool more = false;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        flip_signs(v[i].x);
+        flip_signs(v[i].y);
+        flip_signs(v[i].z);
+        flip_signs(v[i].w);
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t u = 2 * step + h, slot = u % C::kUnits;
-        if (u >= C::kUnits && !wait_done(B, (u - C::kUnits) >> 1, abort, p.err)) return false;
-        uint8_t *dst = smem + slot * kUnit + (r >> 3) * 1024 + (r & 7) * 128;
-        if (h == 1 && tid < kTreeKeys) B->scale[g % kScaleRing][tid] = sc;
+        const uint32_t u = 2 * step + h;
+        if (u >= C::kUnits && !wait_done(B, u - C::kUnits, abort, p.err)) return false;
+        if (h == 0) more = load(w, next_sc, next_step);
+        if (h == 1 && tid < kTreeKeys) scales[g % kScaleRing][tid] = sc;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const uint4 x = v[4 * h + b];
-          *reinterpret_cast<uint4 *>(dst + b * kBox + ((2 * c) ^ (r & 7)) * 16) =
-              make_uint4(s8x2_to_bf16<0>(x.x), s8x2_to_bf16<1>(x.x), s8x2_to_bf16<0>(x.y), s8x2_to_bf16<1>(x.y));
-          *reinterpret_cast<uint4 *>(dst + b * kBox + ((2 * c + 1) ^ (r & 7)) * 16) =
-              make_uint4(s8x2_to_bf16<0>(x.z), s8x2_to_bf16<1>(x.z), s8x2_to_bf16<0>(x.w), s8x2_to_bf16<1>(x.w));
+        for (int i = 0; i < 2; ++i) {
+          const int row = r + 32 * i;
+          uint8_t *dst = smem + (u % C::kUnits) * kUnit + box * kBox + (row >> 3) * 1024 + (row & 7) * 128;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint4 x = v[4 * h + 2 * i + (c >> 1)];
+            const uint2 lo = u8x4_to_bf16(c & 1 ? x.z : x.x), hi = u8x4_to_bf16(c & 1 ? x.w : x.y);
+            *reinterpret_cast<uint4 *>(dst + ((4 * half + c) ^ (row & 7)) * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+          }
         }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B->full[h][step & 3]);
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&B->full[step & 3]);
       ++g;
-      return true;
+      return more;
     };
     uint4 v0[8], v1[8];
     float sc0 = 0.f, sc1 = 0.f;
-    bool more = load(v0, sc0, j0);
-    while (more) {  // the next tile's rows are in flight while this one is stored
-      const bool second = load(v1, sc1, j1);
-      if (!store(v0, sc0, j0) || !second) break;
-      more = load(v0, sc0, j0);
-      if (!store(v1, sc1, j1)) break;
-    }
+    if (it0 < it1 && load(v0, sc0, j0))
+      while (turn(v0, sc0, j0, v1, sc1, j1) && turn(v1, sc1, j1, v0, sc0, j0)) {
+      }
   }
 
   tc_fence_before();

@@ -59,6 +59,7 @@ struct TreeParams {
   const int *cta_item;  // [grid + 1]
   long long rows;
   float scale_log2;
+  int out_32;           // out is 32-byte aligned
   uint32_t *err;
 };
 

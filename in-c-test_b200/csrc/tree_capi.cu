@@ -113,6 +113,7 @@ static int attend(const KvlMlaTreePlan *plan, uint16_t *out, float *lse, const u
     p.cta_item = reinterpret_cast<const int *>(m + plan->off_cta);
     p.rows = rows;
     p.scale_log2 = scale_log2;
+    p.out_32 = (align(out) & 31) == 0;
     p.err = static_cast<uint32_t *>(plan->d_meta);
     cudaError_t e = launch_tree_attend(p, q8, plan->host.grid, s);
     if (e == cudaSuccess)
