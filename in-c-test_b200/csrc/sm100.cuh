@@ -292,23 +292,33 @@ __device__ __forceinline__ void mma_f16_ws_ss(uint32_t d_tmem, uint64_t a_desc, 
       : "memory");
 }
 
-// The same with A read from tensor memory: row r, K packed two 16-bit elements a
-// column, in lane r and again in lane 64 + r (each half of the lanes multiplies
-// its own half of the N columns).  28 cycles at N = 64.
-__device__ __forceinline__ void mma_f16_ws_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                              uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.ws.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
+// 128 rows x 16 bytes from shared memory (a matrix descriptor) into four
+// tensor-memory columns, row r to lane r.
+__device__ __forceinline__ void tmem_cp_128x128b(uint32_t taddr, uint64_t s_desc) {
+  asm volatile("tcgen05.cp.cta_group::1.128x128b [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
 }
 
-// 64 rows x 16 bytes from shared memory (a matrix descriptor) into four
-// tensor-memory columns, row r to lanes r and 64 + r: the A operand above.
-__device__ __forceinline__ void tmem_cp_64x128b_x2(uint32_t taddr, uint64_t s_desc) {
-  asm volatile("tcgen05.cp.cta_group::1.64x128b.warpx2::02_13 [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
+// 16 lanes (from the address's lane, a multiple of 16 in the warp's quarter) x 32
+// columns: value 4 x + 2 y + z of thread l is lane l / 4 + 8 y, column
+// 8 x + 2 (l % 4) + z.
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Four 8 x 8 blocks of 16-bit elements: thread l gives the address of row l % 8
+// of block l / 8 and holds, of every block, row l / 4, elements 2 (l % 4) and + 1.
+__device__ __forceinline__ void stmatrix_x4(uint32_t saddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(saddr), "r"(a), "r"(b),
+               "r"(c), "r"(d)
+               : "memory");
 }
 
 // Arrive (once) on `bar` when all previously issued tcgen05 async ops of this

@@ -292,61 +292,82 @@ namespace treek {
 constexpr uint32_t kBox = kTreeKeys * 128;  // 64 rows x 64 dims bf16 = 8 KB, one SW128 box
 constexpr uint32_t kUnit = 4 * kBox;        // half a tile's latents: 64 rows x 256 dims
 
-// Shared memory and tensor memory.  The score MMA reads its query rows from
-// tensor memory as far as they fit there (kQT boxes of 64 dims), so that shared
-// memory holds three key tiles: while the scores of tile g + 1 run, tile g
-// waits for its P.V and tile g + 2 is on its way.  With the whole query in
-// shared memory and two tiles (scores and P.V of a tile in turn) a tile took
-// 3420 cycles, of which the tensor core worked about 1750.
-//   bf16: scores 32 columns, 7 query boxes in tensor memory, 2 in shared memory
-//   Q8:   scores 64 columns (the latents' part takes the row scale afterwards,
-//         the rope's does not), 6 and 3; two and a half tiles, the converter
-//         warps hold the next one in registers
-template <bool Q8>
-struct Cfg {
-  static constexpr int kUnits = Q8 ? 5 : 6;
-  static constexpr int kQT = Q8 ? 6 : 7, kQS = 9 - kQT;
-  static constexpr uint32_t OFF_R = kUnits * kUnit;  // a tile's rope, until its scores are done
-  static constexpr uint32_t OFF_P = OFF_R + kBox;    // a tile's P, until its P.V is
-  static constexpr uint32_t OFF_QS = OFF_P + kBox;
-  static constexpr uint32_t OFF_BAR = OFF_QS + kQS * kBox;
-  // O (64 rows x 512) takes 256 columns: dims [256 i, 256 i + 128) in columns
-  // [128 i, 128 i + 128) of lanes 0-63, the next 128 dims in lanes 64-127.
-  static constexpr uint32_t kColS = 256, kColQ = kColS + (Q8 ? 64 : 32);
-  static_assert(kColQ + 32 * kQT == 512, "tensor memory");
-};
+// Shared memory holds three key tiles: while the scores of tile g + 1 run, tile g
+// waits for its P.V and tile g + 2 is on its way.  For that the query's latents
+// lie in tensor memory (with the whole query in shared memory and two tiles,
+// scores and P.V of a tile in turn, a tile took 3420 cycles, of which the tensor
+// core worked about 1750).
+constexpr int kUnits = 6;
+constexpr uint32_t OFF_R = kUnits * kUnit;  // ropes of two tiles, until their scores are done
+constexpr uint32_t OFF_P = OFF_R + 2 * kBox;
+constexpr uint32_t OFF_QR = OFF_P + kBox;   // the query's rope box
+constexpr uint32_t OFF_BAR = OFF_QR + kBox;
+
+// Tensor memory, 512 columns x 128 lanes:
+//   O       64 rows x 512, weight-stationary layout, 256 columns: dims [256 i,
+//           256 i + 128) in columns [128 i, 128 i + 128) of lanes 0-63, the next
+//           128 dims in lanes 64-127
+//   scores  plain M = 64 layout: row r in lane 32 (r / 16) + r % 16, the other
+//           half of the lanes free for a second matrix.  A row of A meets the D
+//           of its own lane, so the even query boxes (lanes + 0) and the odd ones
+//           (lanes + 16) give two partial sums, which the softmax adds.  bf16:
+//           two buffers of 64 columns.  Q8: one, and 64 columns for the rope's
+//           part, which the row scale does not touch
+//   query   eight boxes of 64 dims, two to 32 columns
+constexpr uint32_t kColS = 256, kColRope = kColS + 64, kColQ = kColS + 128;
+constexpr uint32_t kOddLanes = 16u << 16;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kU16 = kUnit / 16, kB16 = kBox / 16;  // in units of a matrix descriptor
-constexpr int kScaleRing = 4;
+constexpr int kScaleRing = 3;
 
 constexpr int kSoftThreads = 256;    // warps 4-11: softmax and epilogue
-constexpr int kConvertWarp = 12;     // Q8: warps 12-19 load and convert the latents
-constexpr int kConvertThreads = 256;
+constexpr int kConvertWarp = 12;       // Q8: warps 12-27 load and convert the latents,
+constexpr int kConvertThreads = 256;   // 256 threads a CTA's even tiles, 256 the odd ones
 template <bool Q8>
-constexpr int threads() { return 128 + kSoftThreads + (Q8 ? kConvertThreads : 0); }
+constexpr int threads() { return 128 + kSoftThreads + (Q8 ? 2 * kConvertThreads : 0); }
 
 struct Bars {
   // of step j's unit h: [h][j % 4], phase j / 4.  full: its bytes are there; done:
   // its half of the P.V (its copy to tensor memory) is, so its place is free
+  // (unit 1: and the tile's rope)
   uint64_t full[2][4], done[2][4];
-  uint64_t rope_full;
-  uint64_t qs_full, q_done;  // q_done: the item's last scores are done
-  uint64_t s_full, s_empty;
+  uint64_t qr_full, q_done;        // q_done: the item's last scores are done
+  uint64_t s_full[2], s_empty[2];  // of tile g: [g % 2], phase g / 2
   uint64_t p_full, o_empty, drain[2];
   uint32_t tmem_base;
   int abort;
   uint32_t nonfinite[8];
-  float red[2][kSoftThreads];  // row maxima, row sums: alternate exchanges
+  float red[2][2][kTreeRows];  // row maxima or sums of the two key halves, alternate exchanges
+  float alpha[kTreeRows];
 };
 typedef float Scales[kScaleRing][kTreeKeys];  // Q8, behind Bars: row scales of the tiles in flight
 template <bool Q8>
-constexpr uint32_t smem_bytes() { return Cfg<Q8>::OFF_BAR + sizeof(Bars) + (Q8 ? sizeof(Scales) : 0); }
+constexpr uint32_t smem_bytes() { return OFF_BAR + sizeof(Bars) + (Q8 ? sizeof(Scales) : 0); }
 static_assert(smem_bytes<false>() <= 232448 && smem_bytes<true>() <= 232448, "shared memory budget");
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Packed pairs of fp32: one instruction for two operations.
+__device__ __forceinline__ uint64_t pair_bits(float2 a) { return *reinterpret_cast<const uint64_t *>(&a); }
+__device__ __forceinline__ float2 pair_of(uint64_t a) { return *reinterpret_cast<const float2 *>(&a); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+  return pair_of(d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+  return pair_of(d);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(pair_bits(a)), "l"(pair_bits(b)), "l"(pair_bits(c)));
+  return pair_of(d);
 }
 
 // Matrix descriptor of a SW128 operand from its low word; the high word (8-row
@@ -386,21 +407,20 @@ __device__ __forceinline__ void load_32(const int8_t *src, bool aligned, uint4 &
       : "l"(src));
 }
 
-// Four int8 b as bf16, exactly, from u = b + 128 in 0..255 (flip_signs).  The bf16
-// 0x4300 + u is f = 128 + u for u < 128 and 256 + 2 (u - 128) above, so f - 256
-// is b, or 2 b where b > 0; relu(f / 2 - 128) is what is too much.  Three
-// operations of a pair go to the fp16 pipe and 1.5 to the integer pipe, which is
-// half as fast and bound a form with masks (4 x 32768 rows 10 % slower).
-__device__ __forceinline__ void flip_signs(uint32_t &w) { asm volatile("xor.b32 %0, %0, 0x80808080;" : "+r"(w)); }
-__device__ __forceinline__ uint2 u8x4_to_bf16(uint32_t u) {
+// Four int8 b as bf16, exactly.  With u = b + 128 in 0..255, the bf16 0x4300 + u
+// is f = 128 + u for u < 128 and 256 + 2 (u - 128) above, so f - 256 is b, or 2 b
+// where b > 0; relu(f / 2 - 128) is what is too much.  Three operations of a pair
+// go to the fp16 pipe and 1.5 to the integer pipe.
+__device__ __forceinline__ uint2 s8x4_to_bf16(uint32_t w) {
+  const uint32_t u = w ^ 0x80808080u;
   const uint32_t f[2] = {__byte_perm(u, 0x43434343u, 0x5140), __byte_perm(u, 0x43434343u, 0x5342)};
   uint32_t x[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162 *>(&f[i]);
-    const __nv_bfloat162 over = __hfma2_relu(v, __floats2bfloat162_rn(0.5f, 0.5f), __floats2bfloat162_rn(-128.f, -128.f));
-    const __nv_bfloat162 d = __hsub2(__hsub2(v, __floats2bfloat162_rn(256.f, 256.f)), over);
-    x[i] = *reinterpret_cast<const uint32_t *>(&d);
+    uint32_t d, over;  // constants as bits: 0.5, -128, 256 (a conversion at run time otherwise)
+    asm("fma.rn.relu.bf16x2 %0, %1, %2, %3;" : "=r"(over) : "r"(f[i]), "r"(0x3f003f00u), "r"(0xc300c300u));
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(f[i]), "r"(0x43804380u));
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(x[i]) : "r"(d), "r"(over));
   }
   return make_uint2(x[0], x[1]);
 }
@@ -424,23 +444,22 @@ __device__ __forceinline__ bool wait_full(Bars *B, uint32_t u, volatile int *abo
 //   1, 3   tcgen05 issuers, of the scores and of P.V: a commit holds its thread
 //          until the MMAs before it have left the queue, so one thread for both
 //          leaves the tensor core idle 500 of a tile's 2150 cycles
-//   2      loader of the query boxes that stay in shared memory
-//   4-11   softmax and epilogue: thread t has query row t % 64 and, of a tile's
-//          keys, 32 (t / 64 % 2) + 16 (t / 128) .. + 15 (.ws puts keys 32 and up
-//          into lanes 64-127); of O, the columns 128 (t / 128) .. + 127.  Four
-//          warps took 2500 cycles a Q8 tile and were what bounded it.
-//   12-19  Q8: latents from global memory, as bf16 into the ring
+//   2      loader of the query's rope box
+//   4-11   softmax and epilogue.  Scores: warp w has node w % 4 of the group (its
+//          16 heads) and the keys 32 ((w - 4) / 4) .. + 31 of a tile; thread l the
+//          heads l / 4 and + 8 and eight of the keys (tmem_ld_16x32).  O: thread l
+//          has row 32 (w % 2) + l and 128 columns.  With four warps the softmax of
+//          a Q8 tile took 2500 cycles and bounded the kernel.
+//   12-27  Q8: latents from global memory, as bf16 into the ring
 //
 // The latent ring runs in steps of two units, half a tile each.  An item is a
 // step of query boxes, which the issuer copies to tensor memory (tcgen05.cp),
-// then one step a tile.  The rope box has one place: it is loaded when the
-// scores before are done, from L2, where it was brought with the latents.
+// then one step a tile.
 template <bool Q8>
 __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __grid_constant__ TreeParams p) {
-  using C = Cfg<Q8>;
   extern __shared__ __align__(1024) uint8_t smem[];
-  Bars *B = reinterpret_cast<Bars *>(smem + C::OFF_BAR);
-  Scales &scales = *reinterpret_cast<Scales *>(smem + C::OFF_BAR + sizeof(Bars));
+  Bars *B = reinterpret_cast<Bars *>(smem + OFF_BAR);
+  Scales &scales = *reinterpret_cast<Scales *>(smem + OFF_BAR + sizeof(Bars));
   const uint32_t s_base = smem_u32(smem);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -451,14 +470,15 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
   if (threadIdx.x == 0) {
     for (int h = 0; h < 2; ++h)
       for (int i = 0; i < 4; ++i) {
-        mbar_init(&B->full[h][i], Q8 ? kConvertThreads / 32 : 1);
+        mbar_init(&B->full[h][i], Q8 ? kConvertThreads / 32 + h : 1);  // + 1: the rope's
         mbar_init(&B->done[h][i], 1);
       }
-    mbar_init(&B->rope_full, 1);
-    mbar_init(&B->qs_full, 1);
+    mbar_init(&B->qr_full, 1);
     mbar_init(&B->q_done, 1);
-    mbar_init(&B->s_full, 1);
-    mbar_init(&B->s_empty, kSoftThreads / 32);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&B->s_full[i], 1);
+      mbar_init(&B->s_empty[i], kSoftThreads / 32);
+    }
     mbar_init(&B->p_full, kSoftThreads / 32);
     mbar_init(&B->o_empty, kSoftThreads / 32);
     mbar_init(&B->drain[0], 1);
@@ -481,8 +501,9 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
   const bool fit = !*abort;  // the same for all threads
   asm volatile("griddepcontrol.launch_dependents;");
 
-  // Q8: 640 threads start with 96 registers each; 96 + 2 x 80 + 2 x 112 = 5 x 96
+  // Q8: 896 threads start with 72 registers each; 56 + 2 x 96 + 4 x 64 = 7 x 72
   if (warp < 4) {
+    if (Q8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0 && fit) {
       if (elect_one()) {
         tma_prefetch_desc(&p.tm_q);
@@ -492,7 +513,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
         // the places of step j: their last steps must be done
         auto free_unit = [&](int h) -> bool {
           const uint32_t u = 2 * j + h;
-          return u < C::kUnits || wait_done(B, u - C::kUnits, abort, p.err);
+          return u < kUnits || wait_done(B, u - kUnits, abort, p.err);
         };
         TreeItem nx = p.items[it0];  // descriptors are read one item ahead
         for (int it = it0; it < it1 && ok; ++it) {
@@ -501,32 +522,33 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
           for (int h = 0; h < 2 && ok; ++h) {
             ok = free_unit(h);
             if (!ok) break;
+            // two pairs of boxes; a pair's rows alternate, 16 of the even box
+            // and 16 of the odd one, as their lanes do
             uint64_t *full = &B->full[h][j & 3];
-            mbar_arrive_expect_tx(full, (h ? C::kQT - 4 : 4) * kBox);
-            for (int b = 4 * h; b < (h ? C::kQT : 4); ++b)
-              tma_load_2d(smem + ((2 * j + h) % C::kUnits) * kUnit + (b & 3) * kBox, &p.tm_q, full, 64 * b,
-                          im.node0 * kHeads);
-            if (Q8)  // the barrier counts the converter warps
-              for (int i = 1; i < kConvertThreads / 32; ++i) mbar_arrive(full);
+            mbar_arrive_expect_tx(full, im.nn * 4 * 2048);
+            for (int b = 0; b < 4; ++b)
+              for (int n = 0; n < im.nn; ++n)
+                tma_load_2d(smem + ((2 * j + h) % kUnits) * kUnit + (b >> 1) * 2 * kBox + (2 * n + (b & 1)) * 2048,
+                            &p.tm_q, full, 64 * (4 * h + b), (im.node0 + n) * kHeads);
+            if (Q8)  // the barrier counts the converter warps, and the rope's arrival
+              for (int i = 1; i < kConvertThreads / 32 + h; ++i) mbar_arrive(full);
           }
           if (!ok) break;
           ++j;
           for (int t = im.tile0; t < im.tile1 && ok; ++t, ++g, ++j) {
             const int32_t y = static_cast<int32_t>(im.row0 + static_cast<long long>(kTreeKeys) * t);
-            const int32_t x_rope = Q8 ? 0 : kLatent;
-            if (g > 0) tma_prefetch_l2_2d(&p.tm_kv, x_rope, y);
             for (int h = 0; h < 2 && ok && !Q8; ++h) {
               ok = free_unit(h);
               if (!ok) break;
               uint64_t *full = &B->full[h][j & 3];
-              mbar_arrive_expect_tx(full, kUnit);
+              mbar_arrive_expect_tx(full, kUnit + h * kBox);
               for (int b = 4 * h; b < 4 * h + 4; ++b)
-                tma_load_2d(smem + ((2 * j + h) % C::kUnits) * kUnit + (b & 3) * kBox, &p.tm_kv, full, 64 * b, y);
+                tma_load_2d(smem + ((2 * j + h) % kUnits) * kUnit + (b & 3) * kBox, &p.tm_kv, full, 64 * b, y);
             }
-            if (ok && g > 0) ok = mbar_wait(&B->s_full, (g - 1) & 1, abort, p.err, ERR_TIMEOUT_EMPTY);
+            if (ok && g >= 2) ok = mbar_wait(&B->s_full[g & 1], ((g >> 1) & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY);
             if (!ok) break;
-            mbar_arrive_expect_tx(&B->rope_full, kBox);
-            tma_load_2d(smem + C::OFF_R, &p.tm_kv, &B->rope_full, x_rope, y);
+            if (Q8) mbar_arrive_expect_tx(&B->full[1][j & 3], kBox);
+            tma_load_2d(smem + OFF_R + (g & 1) * kBox, &p.tm_kv, &B->full[1][j & 3], Q8 ? 0 : kLatent, y);
           }
         }
         if (!ok) {  // copies in flight land before the CTA exits; no barrier tells of a half-issued step
@@ -554,53 +576,49 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
-          for (int b = 0; b < C::kQT; ++b)
+          for (int b = 0; b < 4; ++b)
 #pragma unroll
             for (int c = 0; c < 8; ++c)
-              tmem_cp_64x128b_x2(tmem + C::kColQ + 32 * b + 4 * c,
-                                 desc_of(k_lo + ((2 * j + (b >> 2)) % C::kUnits) * kU16 + (b & 3) * kB16 + c));
+              tmem_cp_128x128b(tmem + kColQ + 32 * b + 4 * c,
+                               desc_of(k_lo + ((2 * j + (b >> 1)) % kUnits) * kU16 + (b & 1) * 2 * kB16 + c));
           mma_commit(&B->done[0][j & 3]);
           mma_commit(&B->done[1][j & 3]);
           ++j;
           for (int t = t0; t < t1; ++t, ++j, ++g) {
             // ---- S = Q . K^T
-            ok = wait_full(B, 2 * j, abort, p.err) &&
-                 mbar_wait(&B->s_empty, (g & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY);
-            if (ok && t == t0) ok = mbar_wait(&B->qs_full, n & 1, abort, p.err, ERR_TIMEOUT_FULL);
+            ok = wait_full(B, 2 * j, abort, p.err);
+            // the place of the scores is free: bf16 those of tile g - 2, Q8 of tile g - 1
+            const uint32_t before = Q8 ? g - 1 : g - 2;
+            if (ok && g >= (Q8 ? 1 : 2))
+              ok = mbar_wait(&B->s_empty[before & 1], (before >> 1) & 1, abort, p.err, ERR_TIMEOUT_EMPTY);
+            if (ok && t == t0) ok = mbar_wait(&B->qr_full, n & 1, abort, p.err, ERR_TIMEOUT_FULL);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t s_lat = tmem + C::kColS, s_rope = s_lat + (Q8 ? 32 : 0);
-            // opaque, or the compiler keeps all 36 operand addresses in registers across tiles
-            uint32_t tq = tmem + C::kColQ, kl = k_lo;
+            const uint32_t s_lat = tmem + kColS + (Q8 ? 0 : 64 * (g & 1)), s_rope = Q8 ? tmem + kColRope : s_lat;
+            // opaque, or the compiler keeps all operand addresses in registers across tiles
+            uint32_t tq = tmem + kColQ, kl = k_lo;
             asm volatile("" : "+r"(tq), "+r"(kl));
-            bool hi_ok = false, rope_ok = false;
+            bool hi_ok = false;
 #pragma unroll
             for (int b = 0; b < 8; ++b) {
-              const uint32_t s = (2 * j + (b >> 2)) % C::kUnits;
+              const uint32_t s = (2 * j + (b >> 2)) % kUnits, odd = b & 1 ? kOddLanes : 0;
               if (b == 3) hi_ok = mbar_test(&B->full[1][j & 3], (j >> 2) & 1);  // MMAs are queued meanwhile
               if (b == 4) {
                 if (!hi_ok) ok = wait_full(B, 2 * j + 1, abort, p.err);
                 if (!ok) break;
                 tc_fence_after();
               }
-              if (b == 7) rope_ok = mbar_test(&B->rope_full, g & 1);
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk) {
-                const uint64_t kd = desc_of(kl + s * kU16 + (b & 3) * kB16 + kk * 2);
-                if (b < C::kQT)
-                  mma_f16_ws_ts(s_lat, tq + 32 * b + 8 * kk, kd, id_qk, b + kk > 0);
-                else
-                  mma_f16_ws_ss(s_lat, desc_of(kl + C::OFF_QS / 16 + (b - C::kQT) * kB16 + kk * 2), kd, id_qk, 1u);
-              }
+              for (int kk = 0; kk < 4; ++kk)
+                mma_f16_ts(s_lat + odd, tq + 32 * (b >> 1) + 8 * kk + odd,
+                           desc_of(kl + s * kU16 + (b & 3) * kB16 + kk * 2), id_qk, b > 1 || kk > 0);
             }
-            if (ok && !rope_ok) ok = mbar_wait(&B->rope_full, g & 1, abort, p.err, ERR_TIMEOUT_FULL);
             if (!ok) break;
-            tc_fence_after();
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              mma_f16_ws_ss(s_rope, desc_of(kl + C::OFF_QS / 16 + (8 - C::kQT) * kB16 + kk * 2),
-                            desc_of(kl + C::OFF_R / 16 + kk * 2), id_qk, Q8 ? kk > 0 : 1u);
-            mma_commit(&B->s_full);
+              mma_f16_ss(s_rope, desc_of(kl + OFF_QR / 16 + kk * 2), desc_of(kl + OFF_R / 16 + (g & 1) * kB16 + kk * 2),
+                         id_qk, Q8 ? kk > 0 : 1u);
+            mma_commit(&B->s_full[g & 1]);
             if (t + 1 == t1) mma_commit(&B->q_done);
           }
         }
@@ -611,7 +629,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
     } else if (warp == 3 && fit) {
       if (elect_one()) {
         constexpr uint32_t id_pv = idesc_f16(1, 1, 0, 1, kTreeRows, 256);  // V rows as they lie: MN-major
-        const uint32_t p_lo = desc_lo(s_base + C::OFF_P, 16), v_lo = desc_lo(s_base, kBox);
+        const uint32_t p_lo = desc_lo(s_base + OFF_P, 16), v_lo = desc_lo(s_base, kBox);
         uint32_t g = 0, j = 0;
         bool ok = true;
         int n0 = p.items[it0].tile0, n1 = p.items[it0].tile1;
@@ -634,7 +652,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
             asm volatile("" : "+r"(pl), "+r"(vl));
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint32_t s = (2 * j + h) % C::kUnits;
+              const uint32_t s = (2 * j + h) % kUnits;
 #pragma unroll
               for (int kk = 0; kk < 4; ++kk)
                 mma_f16_ws_ss(tmem + 128 * h, desc_of(pl + kk * 2), desc_of(vl + s * kU16 + kk * 128), id_pv,
@@ -651,149 +669,200 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
         bool ok = true;
         int n = 0;
         for (int it = it0; it < it1; ++it, ++n) {
-          const int node0 = p.items[it].node0;
+          const int node0 = p.items[it].node0, nn = p.items[it].nn;
           if (n > 0) ok = mbar_wait(&B->q_done, (n - 1) & 1, abort, p.err, ERR_TIMEOUT_EMPTY);
           if (!ok) break;
-          mbar_arrive_expect_tx(&B->qs_full, C::kQS * kBox);
-          for (int b = 0; b < C::kQS; ++b)
-            tma_load_2d(smem + C::OFF_QS + b * kBox, &p.tm_q, &B->qs_full, 64 * (C::kQT + b), node0 * kHeads);
+          mbar_arrive_expect_tx(&B->qr_full, nn * 2048);
+          for (int i = 0; i < nn; ++i)
+            tma_load_2d(smem + OFF_QR + i * 2048, &p.tm_q, &B->qr_full, kLatent, (node0 + i) * kHeads);
         }
-        if (!ok) drain_wait(&B->qs_full, (n - 1) & 1, p.err);
+        if (!ok) drain_wait(&B->qr_full, (n - 1) & 1, p.err);
       }
     }
   } else if (warp < kConvertWarp) {
-    if (Q8) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
     if (fit) {
+      const int sub = warp & 3, kh = (warp - 4) >> 2;  // node of the group (lane quarter), half of the keys
       const int tid = threadIdx.x - 128;
-      const int row = tid & 63, half = tid >> 6 & 1, part = tid >> 7;
-      const int key0 = 32 * half + 16 * part;  // the thread's first key of a tile
-      const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+      const int ra = 16 * sub + (lane >> 2), c2 = 2 * (lane & 3);  // rows ra and ra + 8; keys 8 i + c2, + 1 of the half
+      const uint32_t lanes = static_cast<uint32_t>(32 * sub) << 16;
+      const int orow = 32 * (sub & 1) + lane;          // O: the lane's row,
+      const uint32_t ocol = tmem + 128 * kh + lanes;   // its columns,
+      const int odim = 256 * kh + 128 * (sub >> 1);    // and their dims
       uint32_t g = 0, j = 0;
-      bool bad = false;
       uint32_t x = 0;  // exchanges so far
-      // the four values of a row, in the same order for all of its threads
-      auto exchange = [&](float v, float(&r)[4]) {
-        B->red[x & 1][tid] = v;
-        bad = named_bar_or(1, kSoftThreads, bad);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = B->red[x & 1][row + 64 * i];
-        ++x;
-      };
-      auto load_mask = [&](const TreeItem &im) -> uint64_t {
-        return row < im.nn * kHeads ? p.mask[im.node0 + row / kHeads] : 0;
-      };
+      // a negative scale: the scores change their sign as they are read
+      const float scale = fabsf(p.scale_log2);
+      bool bad = false;
+      auto load_mask = [&](const TreeItem &im) -> uint64_t { return sub < im.nn ? p.mask[im.node0 + sub] : 0; };
       TreeItem nx = p.items[it0];  // descriptors and masks are read one item ahead
       uint64_t next_mask = load_mask(nx);
       for (int it = it0; it < it1 && !bad; ++it) {
         const TreeItem im = nx;
         if (it + 1 < it1) nx = p.items[it + 1];
         ++j;  // its query
-        const bool real = row < im.nn * kHeads;
+        const bool real = sub < im.nn;  // or the rows hold whatever was there
         uint64_t mask = next_mask;
         if (im.tree < 64) mask &= (uint64_t(1) << im.tree) - 1;
-        float m = -INFINITY, l = 0.f, r[4];
+        float m[2] = {-INFINITY, -INFINITY};
+        float2 l[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         for (int t = im.tile0; t < im.tile1; ++t, ++g, ++j) {
-          bad |= !mbar_wait(&B->s_full, g & 1, abort, p.err, ERR_TIMEOUT_MMA);
+          bad |= !mbar_wait(&B->s_full[g & 1], (g >> 1) & 1, abort, p.err, ERR_TIMEOUT_MMA);
           tc_fence_after();
-          float s[16];
-          tmem_ld16(tmem + C::kColS + 16 * part + lanes, s);
-          const float *ks = scales[g % kScaleRing] + key0;
-          if (Q8) {
-            float sr[16];
-            tmem_ld16(tmem + C::kColS + 32 + 16 * part + lanes, sr);
-            bad |= !wait_full(B, 2 * j + 1, abort, p.err);  // the converters' row scales
-            tmem_wait_ld();
+          const uint32_t col = tmem + kColS + (Q8 ? 0 : 64 * (g & 1)) + 32 * kh + lanes;
+          float2 ks[4];  // Q8: the keys' row scales
+          float2 s[8];  // [8-key block i][row y]: keys 8 i + c2, + 1
+          {
+            float s0[16], s1[16], sr[Q8 ? 16 : 1];
+            tmem_ld_16x32(col, s0);
+            tmem_ld_16x32(col + kOddLanes, s1);
+            if constexpr (Q8) {
+              tmem_ld_16x32(col + (kColRope - kColS), sr);
+              bad |= !wait_full(B, 2 * j + 1, abort, p.err);  // the converters' row scales
 #pragma unroll
-            for (int c = 0; c < 16; ++c) s[c] = fmaf(s[c], ks[c], sr[c]);
-          } else {
+              for (int i = 0; i < 4; ++i)
+                ks[i] = *reinterpret_cast<const float2 *>(scales[g % kScaleRing] + 32 * kh + c2 + 8 * i);
+            }
             tmem_wait_ld();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&B->s_empty[g & 1]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              s[i] = add2(make_float2(s0[2 * i], s0[2 * i + 1]), make_float2(s1[2 * i], s1[2 * i + 1]));
+            if constexpr (Q8) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) s[i] = fma2(s[i], ks[i >> 1], make_float2(sr[2 * i], sr[2 * i + 1]));
+            }
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&B->s_empty);
           const bool masked = kTreeKeys * (t + 1) > im.len;
-          uint32_t seen = 0xffffu;
+          uint32_t seen = 0xffu;  // bit 2 i + z: key 8 i + c2 + z
           if (masked) {
-            const int d = kTreeKeys * t + key0 - im.len;  // drafted row of the first key
-            seen = d >= 0 ? (d < 64 ? static_cast<uint32_t>(mask >> d) : 0u)
-                          : (d > -16 ? static_cast<uint32_t>(mask << -d) | (0xffffu >> (16 + d)) : 0xffffu);
+            const int d = kTreeKeys * t - im.len;  // drafted row of the tile's first key
+            const uint64_t vis = d >= 0 ? (d < 64 ? mask >> d : 0)
+                                        : (d > -64 ? mask << -d | ((uint64_t(1) << -d) - 1) : ~uint64_t(0));
+            const uint32_t v = static_cast<uint32_t>(vis >> (32 * kh)) >> c2;
+            seen = (v & 3) | (v >> 6 & 12) | (v >> 12 & 48) | (v >> 18 & 192);
             if (!Q8) {
               // A hidden row gets p = 0, but 0 times an infinity or a NaN of the
               // row itself is NaN in the P.V product.  Such a row gives a score
               // that is not finite with every query (a query that is not finite
               // does so with every row, but only its own): clear those rows.
-              uint32_t nf = 0;
+              uint32_t nf[2] = {0, 0};
 #pragma unroll
-              for (int c = 0; c < 16; ++c) nf |= ((__float_as_uint(s[c]) & 0x7f800000u) == 0x7f800000u) ? 1u << c : 0u;
-              if (named_bar_or(2, kSoftThreads, (nf & ~seen) != 0)) {
-                const uint32_t all = __reduce_and_sync(0xffffffffu, nf);
-                if (lane == 0) B->nonfinite[warp - 4] = all;
+              for (int i = 0; i < 8; ++i) {
+                nf[i & 1] |= ((__float_as_uint(s[i].x) & 0x7f800000u) == 0x7f800000u) ? 1u << (2 * (i >> 1)) : 0u;
+                nf[i & 1] |= ((__float_as_uint(s[i].y) & 0x7f800000u) == 0x7f800000u) ? 2u << (2 * (i >> 1)) : 0u;
+              }
+              if (named_bar_or(2, kSoftThreads, ((nf[0] | nf[1]) & ~seen) != 0)) {
+                uint32_t all = nf[0] & nf[1];
+                for (int o = 4; o < 32; o <<= 1) all &= __shfl_xor_sync(0xffffffffu, all, o);
+                uint32_t keys = 0;
+                for (int i = 0; i < 4; ++i) keys |= (all >> 2 * i & 3) << (8 * i + c2);
+                keys = __reduce_or_sync(0xffffffffu, keys);
+                if (lane == 0) B->nonfinite[warp - 4] = keys;
                 named_bar_sync(2, kSoftThreads);
-                uint64_t rows = 0;
-                for (int i = 0; i < 4; ++i)  // half i % 2, part i / 2
-                  rows |= static_cast<uint64_t>(B->nonfinite[2 * i] & B->nonfinite[2 * i + 1])
-                          << (32 * (i & 1) + 16 * (i >> 1));
+                uint32_t rows[2] = {~0u, ~0u};
+                for (int i = 0; i < 8; ++i) rows[i >> 2] &= B->nonfinite[i];
                 const uint32_t box = tid >> 3 & 7;
-                uint8_t *v = smem + ((2 * j + (box >> 2)) % C::kUnits) * kUnit + (box & 3) * kBox + (tid & 7) * 16;
+                uint8_t *v0 = smem + ((2 * j + (box >> 2)) % kUnits) * kUnit + (box & 3) * kBox + (tid & 7) * 16;
                 for (int k = tid >> 6; k < kTreeKeys; k += 4)
-                  if (rows >> k & 1) *reinterpret_cast<uint4 *>(v + k * 128) = make_uint4(0u, 0u, 0u, 0u);
+                  if (rows[k >> 5] >> (k & 31) & 1) *reinterpret_cast<uint4 *>(v0 + k * 128) = make_uint4(0u, 0u, 0u, 0u);
               }
             }
           }
-          float mx = -INFINITY;
+          if (p.scale_log2 < 0.f)
 #pragma unroll
-          for (int c = 0; c < 16; ++c) s[c] *= p.scale_log2;
+            for (int i = 0; i < 8; ++i) s[i] = make_float2(-s[i].x, -s[i].y);
           if (masked)
 #pragma unroll
-            for (int c = 0; c < 16; ++c) s[c] = (seen >> c & 1) ? s[c] : -INFINITY;
+            for (int i = 0; i < 8; ++i) {
+              if (!(seen >> (2 * (i >> 1)) & 1)) s[i].x = -INFINITY;
+              if (!(seen >> (2 * (i >> 1)) & 2)) s[i].y = -INFINITY;
+            }
+          float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < 16; ++c) mx = fmaxf(mx, s[c]);
-          exchange(mx, r);
-          if (bad) break;
-          mx = fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
-          // The reference maximum moves only when a score exceeds it by 2^8; the
-          // four warps of a row decide alike.
-          if (__any_sync(0xffffffffu, mx > m + 8.0f)) {
-            const float mn = fmaxf(m, mx);
-            const float alpha = m == -INFINITY ? 0.f : ex2(m - mn);
+          for (int i = 0; i < 8; ++i) mx[i & 1] = fmaxf(mx[i & 1], fmaxf(s[i].x, s[i].y));
+          // The reference maxima (of the unscaled scores) move only when some row
+          // gets its first score or one that exceeds its by 2^8, then for all rows;
+          // else nothing is exchanged.
+          bool need = false;
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            need |= (mx[y] - m[y]) * scale > 8.0f || (m[y] == -INFINITY && mx[y] > -INFINITY);
+          need &= real;
+          const bool vote = named_bar_or(1, kSoftThreads, need || bad);
+          const uint32_t before = 2 * (t > im.tile0 ? j - 1 : j - 2) + 1;  // the P before is read until its P.V is done
+          const bool p_free = g == 0 || mbar_test(&B->done[1][(before >> 1) & 3], (before >> 3) & 1);
+          if (vote) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              mx[y] = fmaxf(mx[y], __shfl_xor_sync(0xffffffffu, mx[y], 1));
+              mx[y] = fmaxf(mx[y], __shfl_xor_sync(0xffffffffu, mx[y], 2));
+              if ((lane & 3) == 0) B->red[x & 1][kh][ra + 8 * y] = mx[y];
+            }
+            if (named_bar_or(1, kSoftThreads, bad)) {
+              bad = true;
+              break;
+            }
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const float mn = fmaxf(m[y], fmaxf(mx[y], B->red[x & 1][kh ^ 1][ra + 8 * y]));
+              const float alpha = m[y] == -INFINITY ? 0.f : ex2((m[y] - mn) * scale);
+              if (kh == 0 && (lane & 3) == 0) B->alpha[ra + 8 * y] = alpha;
+              l[y] = make_float2(l[y].x * alpha, l[y].y * alpha);
+              m[y] = mn;
+            }
+            ++x;
             if (t > im.tile0) {
               bad |= !wait_done(B, 2 * (j - 1) + 1, abort, p.err);
+              named_bar_sync(1, kSoftThreads);
               tc_fence_after();
+              const float alpha = B->alpha[orow];
 #pragma unroll
               for (int c = 0; c < 128; c += 16) {
                 float o[16];
-                tmem_ld16(tmem + 128 * part + c + lanes, o);
+                tmem_ld16(ocol + c, o);
                 tmem_wait_ld();
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[i] *= alpha;
-                tmem_st16(tmem + 128 * part + c + lanes, o);
+                tmem_st16(ocol + c, o);
               }
               tmem_wait_st();
             }
-            l *= alpha;
-            m = mn;
           }
-          const float ref = m == -INFINITY ? 0.f : m;  // a row that has seen nothing: exp2(-inf) = 0
+          float2 ref[2];  // a row that has seen nothing: exp2(-inf) = 0
 #pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            s[c] = ex2(s[c] - ref);
-            l += s[c];
+          for (int y = 0; y < 2; ++y) {
+            const float r = m[y] == -INFINITY ? 0.f : -m[y] * scale;
+            ref[y] = make_float2(r, r);
           }
+          auto clear_hidden = [&] {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if (!(seen >> (2 * (i >> 1)) & 1)) s[i].x = 0.f;
+              if (!(seen >> (2 * (i >> 1)) & 2)) s[i].y = 0.f;
+            }
+          };
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 e = fma2(s[i], make_float2(scale, scale), ref[i & 1]);
+            s[i] = make_float2(ex2(e.x), ex2(e.y));
+          }
+          if (masked) clear_hidden();  // with a scale of 0 the -inf became NaN
+#pragma unroll
+          for (int i = 0; i < 8; ++i) l[i & 1] = add2(l[i & 1], s[i]);
           if (Q8) {  // O accumulates p * scale * int8 row
 #pragma unroll
-            for (int c = 0; c < 16; ++c) s[c] *= ks[c];
-            if (masked)  // a hidden row's scale may be anything
-#pragma unroll
-              for (int c = 0; c < 16; ++c) s[c] = (seen >> c & 1) ? s[c] : 0.f;
+            for (int i = 0; i < 8; ++i) s[i] = mul2(s[i], ks[i >> 1]);
+            if (masked) clear_hidden();  // a hidden row's scale may be anything
           }
-          // the P before is read until its P.V is done
-          if (g > 0) bad |= !wait_done(B, 2 * (t > im.tile0 ? j - 1 : j - 2) + 1, abort, p.err);
-          uint8_t *pd = smem + C::OFF_P + (row >> 3) * 1024 + (row & 7) * 128;
+          if (!p_free) bad |= !wait_done(B, before, abort, p.err);
+          const uint32_t pd = s_base + OFF_P + 2 * sub * 1024 + (lane & 7) * 128 + (((4 * kh + (lane >> 3)) ^ (lane & 7)) * 16);
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-            *reinterpret_cast<uint4 *>(pd + ((key0 / 8 + c) ^ (row & 7)) * 16) =
-                make_uint4(pack_bf16(s[8 * c], s[8 * c + 1]), pack_bf16(s[8 * c + 2], s[8 * c + 3]),
-                           pack_bf16(s[8 * c + 4], s[8 * c + 5]), pack_bf16(s[8 * c + 6], s[8 * c + 7]));
+          for (int y = 0; y < 2; ++y)
+            stmatrix_x4(pd + y * 1024, pack_bf16(s[y].x, s[y].y), pack_bf16(s[2 + y].x, s[2 + y].y),
+                        pack_bf16(s[4 + y].x, s[4 + y].y), pack_bf16(s[6 + y].x, s[6 + y].y));
           fence_proxy_async_smem();
           tc_fence_before();
           __syncwarp();
@@ -803,13 +872,26 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
         // ---- epilogue
         next_mask = load_mask(nx);
         bad |= !wait_done(B, 2 * (j - 1) + 1, abort, p.err);
-        exchange(l, r);
-        if (bad) break;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          float ly = l[y].x + l[y].y;
+          ly += __shfl_xor_sync(0xffffffffu, ly, 1);
+          ly += __shfl_xor_sync(0xffffffffu, ly, 2);
+          if ((lane & 3) == 0) B->red[x & 1][kh][ra + 8 * y] = ly;
+        }
+        if (named_bar_or(1, kSoftThreads, bad)) {
+          bad = true;
+          break;
+        }
         tc_fence_after();
-        l = (r[0] + r[1]) + (r[2] + r[3]);
-        const float inv = l == 0.f ? 0.f : 1.0f / l;  // nothing seen: out = 0, lse = -inf
-        if (real && tid < kTreeRows) {
-          const float lse = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+        const float(&sum)[2][kTreeRows] = B->red[x & 1];
+        ++x;
+        const float lo = sum[0][orow] + sum[1][orow];
+        const float inv = lo == 0.f ? 0.f : 1.0f / lo;  // nothing seen: out = 0, lse = -inf
+        if (real && kh == 0 && (lane & 3) < 2) {
+          const int y = lane & 1, row = ra + 8 * y;
+          const float lr = sum[0][row] + sum[1][row];
+          const float lse = lr == 0.f ? -INFINITY : ((y ? m[1] : m[0]) * scale + log2f(lr)) * 0.69314718055994531f;
           if (im.slot >= 0)
             p.part_lse[static_cast<size_t>(im.slot) * kTreeRows + row] = lse;
           else if (p.lse)
@@ -818,23 +900,25 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
         // A partial keeps the threads' own layout, [64 column quads][128 lanes]
         // float4: every store of a warp is 512 contiguous bytes.  (Row by row,
         // 16 bytes of 32 different rows a store, an item's end took 13000 cycles.)
+        const bool oreal = orow < im.nn * kHeads;
         float4 *po = reinterpret_cast<float4 *>(p.part_o) +
-                     (static_cast<size_t>(max(im.slot, 0)) * 64 + 32 * part) * 128 + (tid & 127);
-        uint16_t *orow = p.out + (static_cast<size_t>(im.node0) * kHeads + row) * kLatent + 256 * part + 128 * half;
+                     (static_cast<size_t>(max(im.slot, 0)) * 64 + 32 * kh) * 128 + 32 * sub + lane;
+        uint16_t *od = p.out + (static_cast<size_t>(im.node0) * kHeads + orow) * kLatent + odim;
 #pragma unroll
         for (int c = 0; c < 128; c += 16) {
           float o[16];
-          tmem_ld16(tmem + 128 * part + c + lanes, o);
+          tmem_ld16(ocol + c, o);
           tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[i] *= inv;
-          if (im.slot >= 0) {
+          if (oreal && im.slot >= 0) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               po[(c / 4 + i) * 128] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-          } else if (real) {
-            store_bf16x16(orow + c, p.out_32, o);
+          } else if (oreal) {
+            store_bf16x16(od + c, p.out_32, o);
           }
+          __syncwarp();
         }
         tc_fence_before();
         __syncwarp();
@@ -842,85 +926,56 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
       }
     }
   } else if (Q8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
-    if (!fit) it1 = it0;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     // A thread loads 32 latents of a row at a time, four times a tile.  A warp
     // covers 4 rows x 256 dims, eight whole lines: lane bits 3-4 are the box of
     // 64 dims, bits 1-2 the row, bit 0 the half of the box, so that the eight
-    // lanes of a store phase fill the eight 16-byte banks of the swizzle.
-    const int tid = threadIdx.x - 32 * kConvertWarp;
+    // lanes of a store phase fill the eight 16-byte banks of the swizzle.  The
+    // conversion is bound by latencies, not by a pipe: with half as many warps (a
+    // tile by all of them, the next one in registers) a tile took 3500 cycles.
+    const int tid = (threadIdx.x - 32 * kConvertWarp) % kConvertThreads;
+    const uint32_t odd = warp >= kConvertWarp + kConvertThreads / 32;
     const int box = lane >> 3, r = 4 * (tid >> 5) + (lane >> 1 & 3), half = lane & 1;
     const long long last = p.rows - 1;
     const bool aligned = (reinterpret_cast<uintptr_t>(p.lat8) & 31) == 0;
-    // the CTA's tiles in order
-    int it = it0, t = p.items[it0].tile0, t1 = p.items[it0].tile1;
-    long long row0 = p.items[it0].row0;
-    uint32_t j = 0, j0 = 0, j1 = 0;  // steps so far; of the tiles in v0 and v1
-    bool fresh = true;               // the next tile is its item's first: the query's step comes before it
-    // v: [unit][rows r and r + 32]
-    auto load = [&](uint4(&v)[8], float &sc, uint32_t &step) -> bool {
-      if (t >= t1 && ++it < it1) {
-        t = p.items[it].tile0;
-        t1 = p.items[it].tile1;
-        row0 = p.items[it].row0;
-        fresh = true;
-      }
-      if (it >= it1) return false;
-      if (fresh) ++j;
-      fresh = false;
-      step = j++;
-      const long long first = row0 + static_cast<long long>(kTreeKeys) * t;
-      if (tid < kTreeKeys) sc = __ldg(p.lscale + min(first + tid, last));
+    uint32_t j = 0, g = 0;
+    bool ok = fit;
+    for (int it = it0; it < it1 && ok; ++it) {
+      const long long row0 = p.items[it].row0;
+      const int t0 = p.items[it].tile0, t1 = p.items[it].tile1;
+      ++j;  // the query
+      for (int t = t0; t < t1 && ok; ++t, ++j, ++g) {
+        if ((g & 1) != odd) continue;
+        const long long first = row0 + static_cast<long long>(kTreeKeys) * t;
+        const float sc = tid < kTreeKeys ? __ldg(p.lscale + min(first + tid, last)) : 0.f;
+        uint4 v[8];  // [unit][rows r and r + 32]
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        load_32(p.lat8 + min(first + r + 32 * (i & 1), last) * kLatent + (4 * (i >> 1) + box) * 64 + half * 32,
-                aligned, v[2 * i], v[2 * i + 1]);
-      ++t;
-      return true;
-    };
-    uint32_t g = 0;
-    // Stores the tile in v and loads the next one into w; false at the end.  The
-    // next loads are issued only once v has arrived (the sign flips touch all of
-    // it): loads in flight share a scoreboard, and waiting for v with w's behind
-    // it waited for w too, 1100 of 3400 cycles a tile.
-    auto turn = [&](uint4(&v)[8], float sc, uint32_t step, uint4(&w)[8], float &next_sc, uint32_t &next_step) -> bool {
-      bool more = false;
+        for (int i = 0; i < 4; ++i)
+          load_32(p.lat8 + min(first + r + 32 * (i & 1), last) * kLatent + (4 * (i >> 1) + box) * 64 + half * 32,
+                  aligned, v[2 * i], v[2 * i + 1]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        flip_signs(v[i].x);
-        flip_signs(v[i].y);
-        flip_signs(v[i].z);
-        flip_signs(v[i].w);
-      }
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t u = 2 * j + h;
+          if (ok && u >= kUnits) ok = wait_done(B, u - kUnits, abort, p.err);
+          if (!ok) break;
+          if (h == 1 && tid < kTreeKeys) scales[g % kScaleRing][tid] = sc;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t u = 2 * step + h;
-        if (u >= C::kUnits && !wait_done(B, u - C::kUnits, abort, p.err)) return false;
-        if (h == 0) more = load(w, next_sc, next_step);
-        if (h == 1 && tid < kTreeKeys) scales[g % kScaleRing][tid] = sc;
+          for (int i = 0; i < 2; ++i) {
+            const int row = r + 32 * i;
+            uint8_t *dst = smem + (u % kUnits) * kUnit + box * kBox + (row >> 3) * 1024 + (row & 7) * 128;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int row = r + 32 * i;
-          uint8_t *dst = smem + (u % C::kUnits) * kUnit + box * kBox + (row >> 3) * 1024 + (row & 7) * 128;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint4 x = v[4 * h + 2 * i + (c >> 1)];
-            const uint2 lo = u8x4_to_bf16(c & 1 ? x.z : x.x), hi = u8x4_to_bf16(c & 1 ? x.w : x.y);
-            *reinterpret_cast<uint4 *>(dst + ((4 * half + c) ^ (row & 7)) * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            for (int c = 0; c < 4; ++c) {
+              const uint4 x = v[4 * h + 2 * i + (c >> 1)];
+              const uint2 lo = s8x4_to_bf16(c & 1 ? x.z : x.x), hi = s8x4_to_bf16(c & 1 ? x.w : x.y);
+              *reinterpret_cast<uint4 *>(dst + ((4 * half + c) ^ (row & 7)) * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            }
           }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&B->full[h][j & 3]);
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&B->full[h][step & 3]);
       }
-      ++g;
-      return more;
-    };
-    uint4 v0[8], v1[8];
-    float sc0 = 0.f, sc1 = 0.f;
-    if (it0 < it1 && load(v0, sc0, j0))
-      while (turn(v0, sc0, j0, v1, sc1, j1) && turn(v1, sc1, j1, v0, sc0, j0)) {
-      }
+    }
   }
 
   tc_fence_before();

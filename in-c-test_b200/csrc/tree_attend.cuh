@@ -47,7 +47,7 @@ struct TreeMerge {
 
 struct TreeParams {
   CUtensorMap tm_kv;    // bf16 pool [rows][576], or the Q8 pool's rope [rows][64]: 64 x 64 boxes
-  CUtensorMap tm_q;     // q [nodes * 16][576]: 64 x 64 boxes
+  CUtensorMap tm_q;     // q [nodes * 16][576]: 64 dims x 16 rows boxes
   const int8_t *lat8;   // Q8 pool
   const float *lscale;
   const uint64_t *mask; // [nodes]

@@ -96,7 +96,7 @@ static int attend(const KvlMlaTreePlan *plan, uint16_t *out, float *lse, const u
     const bool q8 = !kv;
     const bool maps =
         make_tmap_2d(&p.tm_q, q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kRow, (uint64_t)plan->host.nodes * kHeads, kRow * 2,
-                     64, kTreeRows, CU_TENSOR_MAP_SWIZZLE_128B) &&
+                     64, kHeads, CU_TENSOR_MAP_SWIZZLE_128B) &&
         (q8 ? make_tmap_2d(&p.tm_kv, rope16, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kRope, rows, kRope * 2, 64, kTreeKeys,
                            CU_TENSOR_MAP_SWIZZLE_128B)
             : make_tmap_2d(&p.tm_kv, kv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kRow, rows, kRow * 2, 64, kTreeKeys,
