@@ -64,6 +64,22 @@ bool make_tmap_3d(CUtensorMap *m, const void *base, CUtensorMapDataType dt, cons
   return r == CUDA_SUCCESS;
 }
 
+bool make_tmap_nd(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int rank, const uint64_t *dims,
+                  const uint64_t *strides_bytes, const uint32_t *box, CUtensorMapSwizzle sw) {
+  auto fn = encode_fn();
+  if (!fn || rank < 1 || rank > 5) return false;
+  cuuint64_t d[5], s[4];
+  cuuint32_t b[5], e[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    e[i] = 1;
+    if (i + 1 < rank) s[i] = strides_bytes[i];
+  }
+  return fn(m, dt, rank, const_cast<void *>(base), d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // ------------------------------------------------------------------ plan
 int build_attend_plan(HostPlan &hp, int batch, const int *seq_len, const long long *seq_row0,
                       int max_ctas) {

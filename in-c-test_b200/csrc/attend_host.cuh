@@ -79,6 +79,10 @@ bool make_tmap_2d(CUtensorMap *m, const void *base, CUtensorMapDataType dt, uint
                   uint64_t rows, uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_rows,
                   CUtensorMapSwizzle sw);
 
+// Any rank up to 5; strides_bytes: of the dimensions from the second on.
+bool make_tmap_nd(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int rank, const uint64_t *dims,
+                  const uint64_t *strides_bytes, const uint32_t *box, CUtensorMapSwizzle sw);
+
 cudaError_t launch_merge(float *out, float *lse, const float *part_o, const float *part_lse,
                          const MergeEntry *d_entries, int n_entries, int nh, int R,
                          cudaStream_t stream, int max_count);

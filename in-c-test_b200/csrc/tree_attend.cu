@@ -6,6 +6,7 @@
 #include <queue>
 
 #include "attend_host.cuh"
+#include "pdl.cuh"
 #include "prof.cuh"
 #include "sm100.cuh"
 #include "tree_attend.cuh"
@@ -71,6 +72,7 @@ int build_tree_plan(TreeHostPlan &hp, int batch, const int *cached_len, const in
     im.tile0 = tile0;
     im.tile1 = tile1;
     im.slot = part ? 0 : -1;
+    im.next = -1;
     d.items.push_back(im);
   };
   auto merge_cost = [&](int slots) { return slots ? kMergeCost + kSlotCost * slots : 0.0; };
@@ -176,13 +178,20 @@ int build_tree_plan(TreeHostPlan &hp, int batch, const int *cached_len, const in
     }
     i0 = i1;
   }
-  hp.cta_item.push_back(0);
-  for (const std::vector<int> &v : of) {
-    if (v.empty()) continue;
-    for (int i : v) hp.items.push_back(best.items[i]);
-    hp.cta_item.push_back((int)hp.items.size());
+  // CTA c's items: number c, then along `next`
+  for (int c = 0; c < ctas; ++c)
+    if (!of[c].empty()) hp.items.push_back(best.items[of[c][0]]);
+  hp.grid = (int)hp.items.size();
+  for (int c = 0, n = 0; c < ctas; ++c) {
+    if (of[c].empty()) continue;
+    int last = n++;
+    for (size_t k = 1; k < of[c].size(); ++k) {
+      hp.items[last].next = (int)hp.items.size();
+      last = (int)hp.items.size();
+      hp.items.push_back(best.items[of[c][k]]);
+    }
+    hp.items[last].next = -1;
   }
-  hp.grid = (int)hp.cta_item.size() - 1;
   return 0;
 }
 
@@ -429,6 +438,21 @@ __device__ __forceinline__ uint2 s8x4_to_bf16(uint32_t w) {
 
 using namespace treek;
 
+// The CTA's items; descriptors are read one item ahead.
+struct Items {
+  const TreeItem *items;
+  TreeItem ahead;
+  bool more = true;
+  __device__ __forceinline__ explicit Items(const TreeItem *p) : items(p), ahead(p[blockIdx.x]) {}
+  __device__ __forceinline__ bool next(TreeItem &im) {
+    if (!more) return false;
+    im = ahead;
+    more = im.next >= 0;
+    if (more) ahead = items[im.next];
+    return true;
+  }
+};
+
 // Waits until unit u = 2 step + half is done (or full).  Steps share four
 // barriers, so nobody may ask for a step that is four or more behind the last
 // one loaded.
@@ -463,9 +487,53 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
   const uint32_t s_base = smem_u32(smem);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int it0 = p.cta_item[blockIdx.x];
-  int it1 = p.cta_item[blockIdx.x + 1];
   volatile int *abort = &B->abort;
+
+  // ---- the producer (thread 0): one step a call, false at the end
+  TreeItem pim;
+  pim.next = blockIdx.x;
+  pim.tile1 = 0;
+  int pt = 0;
+  uint32_t pg = 0, pj = 0;  // tiles and steps issued
+  auto produce = [&]() -> bool {
+    // the places of step pj: their last steps must be done
+    auto free_unit = [&](int h) -> bool {
+      const uint32_t u = 2 * pj + h;
+      return u < kUnits || wait_done(B, u - kUnits, abort, p.err);
+    };
+    if (pt == pim.tile1) {
+      if (pim.next < 0) return false;
+      pim = p.items[pim.next];
+      pt = pim.tile0;
+      for (int h = 0; h < 2; ++h) {
+        if (!free_unit(h)) return false;
+        // two pairs of boxes; a pair's rows alternate, 16 of the even box and 16
+        // of the odd one, as their lanes do
+        uint64_t *full = &B->full[h][pj & 3];
+        mbar_arrive_expect_tx(full, kUnit);
+        for (int b = 0; b < 2; ++b)
+          tma_load_5d(smem + ((2 * pj + h) % kUnits) * kUnit + b * 2 * kBox, &p.tm_q, full, 0, 0, 0, 2 * h + b, pim.node0);
+        if (Q8)  // the barrier counts the converter warps, and the rope's arrival
+          for (int i = 1; i < kConvertThreads / 32 + h; ++i) mbar_arrive(full);
+      }
+      ++pj;
+      return true;
+    }
+    const int32_t y = static_cast<int32_t>(pim.row0 + static_cast<long long>(kTreeKeys) * pt);
+    for (int h = 0; h < 2 && !Q8; ++h) {
+      if (!free_unit(h)) return false;
+      uint64_t *full = &B->full[h][pj & 3];
+      mbar_arrive_expect_tx(full, kUnit + h * kBox);
+      tma_load_3d(smem + ((2 * pj + h) % kUnits) * kUnit, &p.tm_lat, full, 0, y, 4 * h);
+    }
+    if (pg >= 2 && !mbar_wait(&B->s_full[pg & 1], ((pg >> 1) & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY)) return false;
+    if (Q8) mbar_arrive_expect_tx(&B->full[1][pj & 3], kBox);
+    tma_load_2d(smem + OFF_R + (pg & 1) * kBox, &p.tm_rope, &B->full[1][pj & 3], Q8 ? 0 : kLatent, y);
+    ++pt;
+    ++pg;
+    ++pj;
+    return true;
+  };
 
   if (threadIdx.x == 0) {
     for (int h = 0; h < 2; ++h)
@@ -489,6 +557,14 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
       atomicOr(p.err, ERR_BAD_PARAM);
     }
     fence_barrier_init();
+    // The first loads go out before the CTA's set-up is done; nothing but the
+    // plan is read before the kernel ahead of this one on the stream is complete.
+    tma_prefetch_desc(&p.tm_q);
+    tma_prefetch_desc(&p.tm_rope);
+    if (!Q8) tma_prefetch_desc(&p.tm_lat);
+    pdl_wait();
+    for (int i = 0; i < 2 && !B->abort; ++i)  // the query and a tile: their places are free
+      if (!produce()) break;
   }
   if (warp == 1) {
     tmem_alloc(&B->tmem_base, kTmemCols);
@@ -499,59 +575,16 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
   tc_fence_after();
   const uint32_t tmem = B->tmem_base;
   const bool fit = !*abort;  // the same for all threads
-  asm volatile("griddepcontrol.launch_dependents;");
+  pdl_wait();
+  pdl_trigger();
 
-  // Q8: 896 threads start with 72 registers each; 56 + 2 x 96 + 4 x 64 = 7 x 72
+  // Q8: 896 threads start with 72 registers each; 72 + 2 x 88 + 4 x 64 = 7 x 72
   if (warp < 4) {
-    if (Q8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 0 && fit) {
-      if (elect_one()) {
-        tma_prefetch_desc(&p.tm_q);
-        tma_prefetch_desc(&p.tm_kv);
-        uint32_t g = 0, j = 0;
-        bool ok = true;
-        // the places of step j: their last steps must be done
-        auto free_unit = [&](int h) -> bool {
-          const uint32_t u = 2 * j + h;
-          return u < kUnits || wait_done(B, u - kUnits, abort, p.err);
-        };
-        TreeItem nx = p.items[it0];  // descriptors are read one item ahead
-        for (int it = it0; it < it1 && ok; ++it) {
-          const TreeItem im = nx;
-          if (it + 1 < it1) nx = p.items[it + 1];
-          for (int h = 0; h < 2 && ok; ++h) {
-            ok = free_unit(h);
-            if (!ok) break;
-            // two pairs of boxes; a pair's rows alternate, 16 of the even box
-            // and 16 of the odd one, as their lanes do
-            uint64_t *full = &B->full[h][j & 3];
-            mbar_arrive_expect_tx(full, im.nn * 4 * 2048);
-            for (int b = 0; b < 4; ++b)
-              for (int n = 0; n < im.nn; ++n)
-                tma_load_2d(smem + ((2 * j + h) % kUnits) * kUnit + (b >> 1) * 2 * kBox + (2 * n + (b & 1)) * 2048,
-                            &p.tm_q, full, 64 * (4 * h + b), (im.node0 + n) * kHeads);
-            if (Q8)  // the barrier counts the converter warps, and the rope's arrival
-              for (int i = 1; i < kConvertThreads / 32 + h; ++i) mbar_arrive(full);
-          }
-          if (!ok) break;
-          ++j;
-          for (int t = im.tile0; t < im.tile1 && ok; ++t, ++g, ++j) {
-            const int32_t y = static_cast<int32_t>(im.row0 + static_cast<long long>(kTreeKeys) * t);
-            for (int h = 0; h < 2 && ok && !Q8; ++h) {
-              ok = free_unit(h);
-              if (!ok) break;
-              uint64_t *full = &B->full[h][j & 3];
-              mbar_arrive_expect_tx(full, kUnit + h * kBox);
-              for (int b = 4 * h; b < 4 * h + 4; ++b)
-                tma_load_2d(smem + ((2 * j + h) % kUnits) * kUnit + (b & 3) * kBox, &p.tm_kv, full, 64 * b, y);
-            }
-            if (ok && g >= 2) ok = mbar_wait(&B->s_full[g & 1], ((g >> 1) & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY);
-            if (!ok) break;
-            if (Q8) mbar_arrive_expect_tx(&B->full[1][j & 3], kBox);
-            tma_load_2d(smem + OFF_R + (g & 1) * kBox, &p.tm_kv, &B->full[1][j & 3], Q8 ? 0 : kLatent, y);
-          }
+      if (lane == 0) {
+        while (produce()) {
         }
-        if (!ok) {  // copies in flight land before the CTA exits; no barrier tells of a half-issued step
+        if (*abort) {  // copies in flight land before the CTA exits; no barrier tells of a half-issued step
           const uint64_t from = globaltimer();
           while (globaltimer() - from < 1000000ull) {
           }
@@ -563,13 +596,10 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
         const uint32_t k_lo = desc_lo(s_base, 16);
         uint32_t g = 0, j = 0;
         bool ok = true;
-        int n0 = p.items[it0].tile0, n1 = p.items[it0].tile1;  // read one item ahead
-        for (int it = it0, n = 0; it < it1 && ok; ++it, ++n) {
-          const int t0 = n0, t1 = n1;
-          if (it + 1 < it1) {
-            n0 = p.items[it + 1].tile0;
-            n1 = p.items[it + 1].tile1;
-          }
+        Items items(p.items);
+        TreeItem im;
+        for (int n = 0; ok && items.next(im); ++n) {
+          const int t0 = im.tile0, t1 = im.tile1;
           // ---- the query's boxes to tensor memory, once the scores before have read theirs
           if (n > 0) ok = mbar_wait(&B->q_done, (n - 1) & 1, abort, p.err, ERR_TIMEOUT_MMA);
           if (ok) ok = wait_full(B, 2 * j, abort, p.err) && wait_full(B, 2 * j + 1, abort, p.err);
@@ -632,13 +662,10 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
         const uint32_t p_lo = desc_lo(s_base + OFF_P, 16), v_lo = desc_lo(s_base, kBox);
         uint32_t g = 0, j = 0;
         bool ok = true;
-        int n0 = p.items[it0].tile0, n1 = p.items[it0].tile1;
-        for (int it = it0, n = 0; it < it1 && ok; ++it, ++n) {
-          const int t0 = n0, t1 = n1;
-          if (it + 1 < it1) {
-            n0 = p.items[it + 1].tile0;
-            n1 = p.items[it + 1].tile1;
-          }
+        Items items(p.items);
+        TreeItem im;
+        for (int n = 0; ok && items.next(im); ++n) {
+          const int t0 = im.tile0, t1 = im.tile1;
           ++j;  // the query
           for (int t = t0; t < t1; ++t, ++j, ++g) {
             // ---- O += P . V
@@ -668,19 +695,20 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
       if (elect_one()) {
         bool ok = true;
         int n = 0;
-        for (int it = it0; it < it1; ++it, ++n) {
-          const int node0 = p.items[it].node0, nn = p.items[it].nn;
+        Items items(p.items);
+        TreeItem im;
+        for (; items.next(im); ++n) {
+          const int node0 = im.node0;
           if (n > 0) ok = mbar_wait(&B->q_done, (n - 1) & 1, abort, p.err, ERR_TIMEOUT_EMPTY);
           if (!ok) break;
-          mbar_arrive_expect_tx(&B->qr_full, nn * 2048);
-          for (int i = 0; i < nn; ++i)
-            tma_load_2d(smem + OFF_QR + i * 2048, &p.tm_q, &B->qr_full, kLatent, (node0 + i) * kHeads);
+          mbar_arrive_expect_tx(&B->qr_full, kBox);
+          tma_load_2d(smem + OFF_QR, &p.tm_qr, &B->qr_full, kLatent, node0 * kHeads);
         }
         if (!ok) drain_wait(&B->qr_full, (n - 1) & 1, p.err);
       }
     }
   } else if (warp < kConvertWarp) {
-    if (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
+    if (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
     if (fit) {
       const int sub = warp & 3, kh = (warp - 4) >> 2;  // node of the group (lane quarter), half of the keys
       const int tid = threadIdx.x - 128;
@@ -694,19 +722,20 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
       // a negative scale: the scores change their sign as they are read
       const float scale = fabsf(p.scale_log2);
       bool bad = false;
-      auto load_mask = [&](const TreeItem &im) -> uint64_t { return sub < im.nn ? p.mask[im.node0 + sub] : 0; };
-      TreeItem nx = p.items[it0];  // descriptors and masks are read one item ahead
-      uint64_t next_mask = load_mask(nx);
-      for (int it = it0; it < it1 && !bad; ++it) {
-        const TreeItem im = nx;
-        if (it + 1 < it1) nx = p.items[it + 1];
+      // the mask word of this warp's node, drafted rows of its sequence only
+      auto load_mask = [&](const TreeItem &im) -> uint64_t {
+        const uint64_t w = sub < im.nn ? p.mask[im.node0 + sub] : 0;
+        return im.tree < 64 ? w & ((uint64_t(1) << im.tree) - 1) : w;
+      };
+      int it = blockIdx.x;
+      uint64_t mask = load_mask(p.items[it]);
+      for (;;) {
         ++j;  // its query
-        const bool real = sub < im.nn;  // or the rows hold whatever was there
-        uint64_t mask = next_mask;
-        if (im.tree < 64) mask &= (uint64_t(1) << im.tree) - 1;
+        const int tile0 = p.items[it].tile0, tile1 = p.items[it].tile1, len = p.items[it].len;
+        const bool real = sub < p.items[it].nn;  // or the rows hold whatever was there
         float m[2] = {-INFINITY, -INFINITY};
         float2 l[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        for (int t = im.tile0; t < im.tile1; ++t, ++g, ++j) {
+        for (int t = tile0; t < tile1; ++t, ++g, ++j) {
           bad |= !mbar_wait(&B->s_full[g & 1], (g >> 1) & 1, abort, p.err, ERR_TIMEOUT_MMA);
           tc_fence_after();
           const uint32_t col = tmem + kColS + (Q8 ? 0 : 64 * (g & 1)) + 32 * kh + lanes;
@@ -735,10 +764,10 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
               for (int i = 0; i < 8; ++i) s[i] = fma2(s[i], ks[i >> 1], make_float2(sr[2 * i], sr[2 * i + 1]));
             }
           }
-          const bool masked = kTreeKeys * (t + 1) > im.len;
+          const bool masked = kTreeKeys * (t + 1) > len;
           uint32_t seen = 0xffu;  // bit 2 i + z: key 8 i + c2 + z
           if (masked) {
-            const int d = kTreeKeys * t - im.len;  // drafted row of the tile's first key
+            const int d = kTreeKeys * t - len;  // drafted row of the tile's first key
             const uint64_t vis = d >= 0 ? (d < 64 ? mask >> d : 0)
                                         : (d > -64 ? mask << -d | ((uint64_t(1) << -d) - 1) : ~uint64_t(0));
             const uint32_t v = static_cast<uint32_t>(vis >> (32 * kh)) >> c2;
@@ -792,7 +821,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
             need |= (mx[y] - m[y]) * scale > 8.0f || (m[y] == -INFINITY && mx[y] > -INFINITY);
           need &= real;
           const bool vote = named_bar_or(1, kSoftThreads, need || bad);
-          const uint32_t before = 2 * (t > im.tile0 ? j - 1 : j - 2) + 1;  // the P before is read until its P.V is done
+          const uint32_t before = 2 * (t > tile0 ? j - 1 : j - 2) + 1;  // the P before is read until its P.V is done
           const bool p_free = g == 0 || mbar_test(&B->done[1][(before >> 1) & 3], (before >> 3) & 1);
           if (vote) {
 #pragma unroll
@@ -814,7 +843,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
               m[y] = mn;
             }
             ++x;
-            if (t > im.tile0) {
+            if (t > tile0) {
               bad |= !wait_done(B, 2 * (j - 1) + 1, abort, p.err);
               named_bar_sync(1, kSoftThreads);
               tc_fence_after();
@@ -870,7 +899,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
         }
         if (bad) break;
         // ---- epilogue
-        next_mask = load_mask(nx);
+        const TreeItem im = p.items[it];
         bad |= !wait_done(B, 2 * (j - 1) + 1, abort, p.err);
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
@@ -884,6 +913,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
           break;
         }
         tc_fence_after();
+        if (im.next >= 0) mask = load_mask(p.items[im.next]);
         const float(&sum)[2][kTreeRows] = B->red[x & 1];
         ++x;
         const float lo = sum[0][orow] + sum[1][orow];
@@ -900,10 +930,15 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
         // A partial keeps the threads' own layout, [64 column quads][128 lanes]
         // float4: every store of a warp is 512 contiguous bytes.  (Row by row,
         // 16 bytes of 32 different rows a store, an item's end took 13000 cycles.)
-        const bool oreal = orow < im.nn * kHeads;
+        // A whole result goes row by row to the output: the CTA's last one through
+        // the ring, which is empty by then, and by TMA (from registers, 32 bytes
+        // of 32 rows a store, it took 6300 cycles); others from registers, while
+        // the ring fills for the next item.
+        const bool oreal = orow < im.nn * kHeads, staged = im.slot < 0 && im.next < 0;
         float4 *po = reinterpret_cast<float4 *>(p.part_o) +
                      (static_cast<size_t>(max(im.slot, 0)) * 64 + 32 * kh) * 128 + 32 * sub + lane;
         uint16_t *od = p.out + (static_cast<size_t>(im.node0) * kHeads + orow) * kLatent + odim;
+        uint8_t *stage = smem + (odim >> 6) * kBox + (orow >> 3) * 1024 + (orow & 7) * 128;
 #pragma unroll
         for (int c = 0; c < 128; c += 16) {
           float o[16];
@@ -911,7 +946,13 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
           tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[i] *= inv;
-          if (oreal && im.slot >= 0) {
+          if (staged) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              *reinterpret_cast<uint4 *>(stage + (c >> 6) * kBox + ((((c & 63) >> 3) + i) ^ (orow & 7)) * 16) =
+                  make_uint4(pack_bf16(o[8 * i], o[8 * i + 1]), pack_bf16(o[8 * i + 2], o[8 * i + 3]),
+                             pack_bf16(o[8 * i + 4], o[8 * i + 5]), pack_bf16(o[8 * i + 6], o[8 * i + 7]));
+          } else if (oreal && im.slot >= 0) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               po[(c / 4 + i) * 128] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
@@ -920,9 +961,21 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
           }
           __syncwarp();
         }
+        if (staged) {
+          fence_proxy_async_smem();
+          named_bar_sync(1, kSoftThreads);
+          if (warp == 4 && lane < im.nn) {
+            for (int b = 0; b < 8; ++b)
+              tma_store_2d(&p.tm_out, smem + b * kBox + lane * 2048, 64 * b, (im.node0 + lane) * kHeads);
+            tma_store_wait_read();
+          }
+          __syncwarp();
+        }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&B->o_empty);
+        if (im.next < 0) break;
+        it = im.next;
       }
     }
   } else if (Q8) {
@@ -940,7 +993,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
     const bool aligned = (reinterpret_cast<uintptr_t>(p.lat8) & 31) == 0;
     uint32_t j = 0, g = 0;
     bool ok = fit;
-    for (int it = it0; it < it1 && ok; ++it) {
+    for (int it = blockIdx.x; it >= 0 && ok; it = p.items[it].next) {
       const long long row0 = p.items[it].row0;
       const int t0 = p.items[it].tile0, t1 = p.items[it].tile1;
       ++j;  // the query
@@ -986,6 +1039,23 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
   }
 }
 
+bool tree_maps(TreeParams &p, const uint16_t *q, const uint16_t *kv, const uint16_t *rope16, uint16_t *out, int nodes,
+               int64_t rows) {
+  const CUtensorMapDataType dt = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUtensorMapSwizzle sw = CU_TENSOR_MAP_SWIZZLE_128B;
+  const uint64_t n = nodes, r = rows, row = kRow * 2;
+  const uint64_t qd[5] = {64, kHeads, 2, 4, n}, qs[4] = {row, 128, 256, kHeads * row};
+  const uint32_t qb[5] = {64, kHeads, 2, 1, kTreeGroup};
+  const uint64_t ld[3] = {64, r, 8}, ls[2] = {row, 128};
+  const uint32_t lb[3] = {64, kTreeKeys, 4};
+  return make_tmap_nd(&p.tm_q, q, dt, 5, qd, qs, qb, sw) &&
+         make_tmap_2d(&p.tm_qr, q, dt, kRow, n * kHeads, row, 64, kTreeRows, sw) &&
+         make_tmap_2d(&p.tm_out, out, dt, kLatent, n * kHeads, kLatent * 2, 64, kHeads, sw) &&
+         (kv ? make_tmap_nd(&p.tm_lat, kv, dt, 3, ld, ls, lb, sw) &&
+                   make_tmap_2d(&p.tm_rope, kv, dt, kRow, r, row, 64, kTreeKeys, sw)
+             : make_tmap_2d(&p.tm_rope, rope16, dt, kRope, r, kRope * 2, 64, kTreeKeys, sw));
+}
+
 cudaError_t launch_tree_attend(const TreeParams &p, bool q8, int grid, cudaStream_t s) {
   static std::atomic<unsigned long long> opted[2];
   const void *fn = q8 ? reinterpret_cast<const void *>(tree_attend_kernel<true>)
@@ -993,44 +1063,47 @@ cudaError_t launch_tree_attend(const TreeParams &p, bool q8, int grid, cudaStrea
   cudaError_t e = smem_opt_in(fn, q8 ? smem_bytes<true>() : smem_bytes<false>(), opted[q8]);
   if (e != cudaSuccess) return e;
   ProfScope ps(q8 ? "tree_attend_q8" : "tree_attend_bf16", s);
-  if (q8)
-    tree_attend_kernel<true><<<grid, threads<true>(), smem_bytes<true>(), s>>>(p);
-  else
-    tree_attend_kernel<false><<<grid, threads<false>(), smem_bytes<false>(), s>>>(p);
-  return cudaGetLastError();
+  if (q8) return launch_dependent(tree_attend_kernel<true>, dim3(grid), dim3(threads<true>()), smem_bytes<true>(), s, p);
+  return launch_dependent(tree_attend_kernel<false>, dim3(grid), dim3(threads<false>()), smem_bytes<false>(), s, p);
 }
 
 // Combines the partials of the split (sequence, group)s:
 //     out = sum_q w_q o_q / sum_q w_q,  w_q = exp(lse_q - max lse),
 //     lse = max lse + log sum_q w_q.
-// Thread (tid, z) of block (entry, quad) has four output dims of one query row,
-// as the attend's thread tid left them, and the parts z, z + Z, ...; the Z
-// sums are added in order.  Bound by reading the partials (L2 mostly).
-template <int Z>
-__global__ void __launch_bounds__(128 * Z) tree_merge_kernel(uint16_t *out, float *lse, const float *part_o,
-                                                             const float *part_lse, const TreeMerge *entries) {
+// Thread (row or lane, z) of block (entry, quad) has four output dims of one
+// query row, as the attend's lane left them, and the parts z, z + Z, ...; the Z
+// sums are added in order.  Bound by the latency of its two passes over a few
+// parts a thread (lse, then outputs); the outputs lie in L2 mostly.
+template <int Z, int LANES, int UNROLL>
+__global__ void __launch_bounds__(LANES * Z) tree_merge_kernel(uint16_t *out, float *lse, const float *part_o,
+                                                               const float *part_lse, const TreeMerge *entries) {
   const TreeMerge e = entries[blockIdx.x];
-  const int tid = threadIdx.x & 127, z = threadIdx.x >> 7, quad = blockIdx.y;
-  const int row = tid & 63, half = tid >> 6;
-  __shared__ float4 acc_z[Z > 1 ? Z : 1][128];
-  __shared__ float max_z[Z][128], sum_z[Z][128];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int tid = threadIdx.x % LANES, z = threadIdx.x / LANES, quad = blockIdx.y;
+  const int at = blockIdx.z * LANES + tid;  // the attend's lane
+  const int row = at & 63, half = at >> 6;
+  __shared__ float4 acc_z[Z][LANES];
+  __shared__ float max_z[Z][LANES], sum_z[Z][LANES];
+  pdl_wait();
+  pdl_trigger();
   const bool real = row < e.nn * kHeads;
   const float *ls = part_lse + static_cast<size_t>(e.first) * kTreeRows + row;
-  const float4 *os = reinterpret_cast<const float4 *>(part_o) + (static_cast<size_t>(e.first) * 64 + quad) * 128 + tid;
+  const float4 *os = reinterpret_cast<const float4 *>(part_o) + (static_cast<size_t>(e.first) * 64 + quad) * 128 + at;
   float m = -INFINITY;
-  if (real)
+  if (real) {
+#pragma unroll UNROLL
     for (int q = z; q < e.count; q += Z) m = fmaxf(m, ls[q * kTreeRows]);
+  }
   if (Z > 1) {
     max_z[z][tid] = m;
     __syncthreads();
+#pragma unroll
     for (int i = 0; i < Z; ++i) m = fmaxf(m, max_z[i][tid]);
   }
   const float ref = m == -INFINITY ? 0.f : m;  // no part has seen a row: all weights are 0
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
   if (real) {
-#pragma unroll 4
+#pragma unroll UNROLL
     for (int q = z; q < e.count; q += Z) {
       const float w = __expf(ls[q * kTreeRows] - ref);
       const float4 v = os[static_cast<size_t>(q) * 64 * 128];
@@ -1059,7 +1132,7 @@ __global__ void __launch_bounds__(128 * Z) tree_merge_kernel(uint16_t *out, floa
   const size_t orow = static_cast<size_t>(e.node0) * kHeads + row;
   if (lse && quad == 0 && half == 0) lse[orow] = sum == 0.f ? -INFINITY : m + logf(sum);
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  const int c = 4 * quad;  // the attend thread's column
+  const int c = 4 * quad;  // the attend lane's column
   *reinterpret_cast<uint2 *>(out + orow * kLatent + (c >> 7) * 256 + half * 128 + (c & 127)) =
       make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
 }
@@ -1067,19 +1140,14 @@ __global__ void __launch_bounds__(128 * Z) tree_merge_kernel(uint16_t *out, floa
 cudaError_t launch_tree_merge(const TreeParams &p, const TreeMerge *entries, int n, int max_count, cudaStream_t s) {
   if (n <= 0) return cudaSuccess;
   ProfScope ps("tree_merge", s);
+  auto launch = [&](auto f, int z, int lanes) {
+    return launch_dependent(f, dim3(n, 64, 128 / lanes), dim3(lanes * z), 0, s, p.out, p.lse, (const float *)p.part_o,
+                            (const float *)p.part_lse, entries);
+  };
   // a few parts a thread: more threads share an entry that has many
-  const int z = max_count <= 8 ? 1 : max_count <= 32 ? 4 : 8;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(n, 64);
-  cfg.blockDim = dim3(128 * z);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  auto f = z == 1 ? tree_merge_kernel<1> : z == 4 ? tree_merge_kernel<4> : tree_merge_kernel<8>;
-  return cudaLaunchKernelEx(&cfg, f, p.out, p.lse, (const float *)p.part_o, (const float *)p.part_lse, entries);
+  if (max_count <= 8) return launch(tree_merge_kernel<1, 128, 8>, 1, 128);
+  if (max_count <= 32) return launch(tree_merge_kernel<4, 128, 8>, 4, 128);
+  return launch(tree_merge_kernel<16, 64, 4>, 16, 64);
 }
 
 }  // namespace kvl

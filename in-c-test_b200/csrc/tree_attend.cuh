@@ -29,7 +29,7 @@ constexpr int kTreeGroup = 4;                          // nodes of a group
 constexpr int kTreeRows = kTreeGroup * kHeads;         // query rows of a group
 constexpr int kTreeKeys = 64;                          // key rows of a tile
 
-struct TreeItem {
+struct alignas(16) TreeItem {
   long long row0;  // pool row of the sequence's row 0
   int len;         // cached rows of the sequence
   int tree;        // its drafted rows
@@ -37,6 +37,7 @@ struct TreeItem {
   int nn;          // nodes of the group (1..4)
   int tile0, tile1;  // tiles [tile0, tile1)
   int slot;        // partial slot, or -1 when the chunk is the whole sequence
+  int next;        // next item of the CTA, or -1; CTA c starts with item c
 };
 
 // The (sequence, group) results that are combined from partials.
@@ -46,8 +47,11 @@ struct TreeMerge {
 };
 
 struct TreeParams {
-  CUtensorMap tm_kv;    // bf16 pool [rows][576], or the Q8 pool's rope [rows][64]: 64 x 64 boxes
-  CUtensorMap tm_q;     // q [nodes * 16][576]: 64 dims x 16 rows boxes
+  CUtensorMap tm_lat;   // bf16 pool: [box of 64 dims][rows][64], 4 x 64 x 64 a load
+  CUtensorMap tm_rope;  // bf16 pool or the Q8 pool's rope, 64 rows x 64
+  CUtensorMap tm_q;     // the query's latents: [node][pair of boxes][odd][16 heads][64], a load: 4 x 1 x 2 x 16 x 64
+  CUtensorMap tm_qr;    // its rope: 64 rows (4 nodes) x 64
+  CUtensorMap tm_out;   // out [nodes * 16][512]: 16 rows x 64 dims
   const int8_t *lat8;   // Q8 pool
   const float *lscale;
   const uint64_t *mask; // [nodes]
@@ -56,7 +60,6 @@ struct TreeParams {
   float *part_o;        // [slots][64][512]
   float *part_lse;      // [slots][64]
   const TreeItem *items;
-  const int *cta_item;  // [grid + 1]
   long long rows;
   float scale_log2;
   int out_32;           // out is 32-byte aligned
@@ -67,7 +70,6 @@ struct TreeParams {
 struct TreeHostPlan {
   int batch = 0, nodes = 0, grid = 0, slots = 0, max_merge = 0;
   std::vector<TreeItem> items;
-  std::vector<int> cta_item;
   std::vector<TreeMerge> merges;
   std::vector<int> len, tree, seq_of_node, first_node;
   std::vector<long long> row0;
@@ -92,6 +94,8 @@ struct TreeGenericParams {
   float scale_log2;
 };
 
+bool tree_maps(TreeParams &p, const uint16_t *q, const uint16_t *kv, const uint16_t *rope16, uint16_t *out, int nodes,
+               int64_t rows);  // kv null: a Q8 pool
 cudaError_t launch_tree_attend(const TreeParams &p, bool q8, int grid, cudaStream_t s);
 cudaError_t launch_tree_merge(const TreeParams &p, const TreeMerge *entries, int n, int max_count, cudaStream_t s);
 cudaError_t launch_tree_generic(const TreeGenericParams &p, int nodes, cudaStream_t s);

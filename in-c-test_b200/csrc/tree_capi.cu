@@ -38,7 +38,6 @@ static int upload(KvlMlaTreePlan &p) {
     size_t *off;
   } parts[] = {
       {h.items.data(), h.items.size() * sizeof(TreeItem), &p.off_items},
-      {h.cta_item.data(), h.cta_item.size() * sizeof(int), &p.off_cta},
       {h.merges.data(), h.merges.size() * sizeof(TreeMerge), &p.off_merge},
       {h.row0.data(), h.row0.size() * sizeof(long long), &p.off_row0},
       {h.len.data(), h.len.size() * sizeof(int), &p.off_len},
@@ -94,14 +93,7 @@ static int attend(const KvlMlaTreePlan *plan, uint16_t *out, float *lse, const u
     TreeParams p;
     std::memset(&p, 0, sizeof p);
     const bool q8 = !kv;
-    const bool maps =
-        make_tmap_2d(&p.tm_q, q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kRow, (uint64_t)plan->host.nodes * kHeads, kRow * 2,
-                     64, kHeads, CU_TENSOR_MAP_SWIZZLE_128B) &&
-        (q8 ? make_tmap_2d(&p.tm_kv, rope16, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kRope, rows, kRope * 2, 64, kTreeKeys,
-                           CU_TENSOR_MAP_SWIZZLE_128B)
-            : make_tmap_2d(&p.tm_kv, kv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, kRow, rows, kRow * 2, 64, kTreeKeys,
-                           CU_TENSOR_MAP_SWIZZLE_128B));
-    if (!maps) return fail("tree attend: tensor map");
+    if (!tree_maps(p, q, kv, rope16, out, plan->host.nodes, rows)) return fail("tree attend: tensor map");
     p.lat8 = lat8;
     p.lscale = lscale;
     p.mask = mask;
@@ -110,7 +102,6 @@ static int attend(const KvlMlaTreePlan *plan, uint16_t *out, float *lse, const u
     p.part_o = static_cast<float *>(plan->d_work);
     p.part_lse = p.part_o + (size_t)plan->host.slots * kTreeRows * kLatent;
     p.items = reinterpret_cast<const TreeItem *>(m + plan->off_items);
-    p.cta_item = reinterpret_cast<const int *>(m + plan->off_cta);
     p.rows = rows;
     p.scale_log2 = scale_log2;
     p.out_32 = (align(out) & 31) == 0;
