@@ -26,7 +26,11 @@ void set_error_text(const char *msg);
 
 constexpr int kMaxPools = 64;
 constexpr int kMaxPath = 64;
-constexpr int kTileBytes = 36 * 1024;  // 32 bf16 rows of 1152 bytes
+constexpr int kMaxRowBytes = 36 * 1024;
+constexpr int kMoveRows = 32;   // of a move tile
+constexpr size_t kMoveSmem = 220 * 1024;  // of the move kernels' blocks on an SM
+constexpr size_t kForkSmem = 84 * 1024;   // of a block that moves runs that do not overlap
+constexpr int kMaxStages = 16;            // move tiles in a block's shared memory
 
 // The arrays of up to 64 pools: base pointers, bytes of a row, and the widest
 // access (16, 8, 4, 2 or 1 bytes) that all rows of all pools are aligned to.
@@ -124,10 +128,12 @@ __global__ void __launch_bounds__(128) tree_accept_kernel(const __grid_constant_
 }
 
 // ------------------------------------------------------------------ move
-struct MoveTile {
-  long long src, dst;
-  int n;
-  int dep;  // compaction: tiles [dep, this) read rows that this tile overwrites
+// `n` rows go from row `src` to row `dst`.  In a compaction the tiles
+// [dep, dep + deps) read rows that this one overwrites.
+struct alignas(16) MoveTile {
+  int src, dst;
+  int dep;
+  uint16_t n, deps;
 };
 
 struct MoveParams {
@@ -135,6 +141,7 @@ struct MoveParams {
   const MoveTile *tiles;
   int n_tiles;
   int compact;
+  int stages;        // ring kernel: tiles in shared memory at once
   uint32_t *ticket;  // compaction: next (pool, tile)
   uint32_t *read;    // compaction: [pools][tiles], 1 once the tile's rows have been read
   uint32_t *err;
@@ -156,12 +163,31 @@ __device__ __forceinline__ void copy_any(int vec, uint8_t *dst, const uint8_t *s
   }
 }
 
+// Waits until flag `d` of a compaction's tiles is set, within the limit.
+__device__ __forceinline__ bool wait_read(const uint32_t *flag) {
+  const uint64_t t0 = globaltimer();
+  for (;;) {
+    uint32_t seen;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(flag) : "memory");
+    if (seen) return true;
+    if (globaltimer() - t0 > KVL_WAIT_LIMIT_NS) return false;
+  }
+}
+
+__device__ __forceinline__ void set_read(uint32_t *flag) {
+  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(flag), "r"(1u) : "memory");
+}
+
 // A tile's rows go through shared memory.  In a compaction the blocks take the
 // tiles in order (a ticket), and a tile is written only once the tiles before
-// it whose sources it overwrites have been read.  Reading never waits, so the
-// lowest tile in flight always gets through; its block holds it already, so no
-// block waits for one that has not started.
-__global__ void __launch_bounds__(256) pool_move_kernel(const __grid_constant__ MoveParams p) {
+// it whose sources it overwrites have been read.  Reading never waits for
+// another block, and a block reads its tiles in the order of their tickets, so
+// the lowest tile not yet written always gets through; its block holds it
+// already, so no block waits for one that has not started.
+
+// Rows that bulk copies cannot move (not a multiple of 16 bytes, or not aligned
+// to 16): one tile at a time through a block's threads.
+__global__ void __launch_bounds__(256) pool_move_any_kernel(const __grid_constant__ MoveParams p) {
   extern __shared__ __align__(16) uint8_t buf[];
   __shared__ uint32_t my;
   const uint32_t total = (uint32_t)p.n_tiles * p.a.pools;
@@ -178,7 +204,7 @@ __global__ void __launch_bounds__(256) pool_move_kernel(const __grid_constant__ 
     int at = 0;
     for (int k = 0; k < p.a.arrays; ++k) {
       const int bytes = tile.n * p.a.row_bytes[k];
-      copy_any(p.a.vec[k], buf + at, p.a.base[k][pool] + tile.src * p.a.row_bytes[k], bytes);
+      copy_any(p.a.vec[k], buf + at, p.a.base[k][pool] + (size_t)tile.src * p.a.row_bytes[k], bytes);
       at += (bytes + 15) & ~15;
     }
     __syncthreads();
@@ -186,16 +212,9 @@ __global__ void __launch_bounds__(256) pool_move_kernel(const __grid_constant__ 
       uint32_t *flags = p.read + (size_t)pool * p.n_tiles;
       if (threadIdx.x == 0) {
         __threadfence();
-        asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(flags + ti), "r"(1u) : "memory");
+        set_read(flags + ti);
       }
-      bool late = false;
-      for (int d = tile.dep + threadIdx.x; d < ti; d += blockDim.x) {
-        const uint64_t t0 = globaltimer();
-        for (uint32_t seen = 0; !seen && !late;) {
-          asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(flags + d) : "memory");
-          late = !seen && globaltimer() - t0 > KVL_WAIT_LIMIT_NS;
-        }
-      }
+      const bool late = (int)threadIdx.x < tile.deps && !wait_read(flags + tile.dep + threadIdx.x);
       if (__syncthreads_or(late)) {  // leave the tile unwritten rather than lose an unread row
         if (threadIdx.x == 0) atomicOr(p.err, ERR_TIMEOUT_FULL);
         continue;
@@ -204,11 +223,141 @@ __global__ void __launch_bounds__(256) pool_move_kernel(const __grid_constant__ 
     at = 0;
     for (int k = 0; k < p.a.arrays; ++k) {
       const int bytes = tile.n * p.a.row_bytes[k];
-      copy_any(p.a.vec[k], p.a.base[k][pool] + tile.dst * p.a.row_bytes[k], buf + at, bytes);
+      copy_any(p.a.vec[k], p.a.base[k][pool] + (size_t)tile.dst * p.a.row_bytes[k], buf + at, bytes);
       at += (bytes + 15) & ~15;
     }
     __syncthreads();
   }
+}
+
+// The same with bulk copies, for arrays of 16-byte rows and arrays of one word
+// a row (the Q8 row scales): one warp reads tiles into a ring, one writes them,
+// and in a compaction one tells that they were read.
+// A tile's reading, the flag that tells of it and its writing overlap those of
+// the tiles before and after it.  Array k of tile slot q lies at q * tile bytes
+// + `kMoveRows` rows of the arrays before it.
+//
+// Two blocks an SM.  What bounds it is DRAM: 27 bf16 pools whose 4096-row prompt
+// goes to four places take 112 us, the same on Q8 61 us, a prompt of 32768 rows
+// once 311 us (at the copy rate: 99, 55 and 316); a pool of 64 sequences of up
+// to 8192 rows compacted 98 us, 27 Q8 pools of 31 sequences of up to 1000 rows
+// 111 us (92 and 80).  With one tile a block in registers' reach, read by its
+// threads and then written, the first took 138 us, the compactions 243 and 250.
+// The depth: a copy that nothing orders wants about 150 KB on its way in an SM
+// (two bf16 tiles a block; five take 121 us, for more is then read and written
+// at once), a compaction all it can get (Q8: two tiles a block 270 us, four 131,
+// five 111), for a tile waits in the ring until the flags of others have come.
+__global__ void __launch_bounds__(96) pool_move_kernel(const __grid_constant__ MoveParams p) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages];
+  __shared__ struct {
+    MoveTile tile;
+    uint32_t t;
+  } slot[kMaxStages];
+  __shared__ volatile int gave_up[2];  // the writing warp still writes what was read when the reading one gave up
+  const int lane = threadIdx.x & 31;
+  const uint32_t total = (uint32_t)p.n_tiles * p.a.pools;
+  const int stages = p.stages;
+  int tile_bytes = 0, bulk_row = 0;
+  for (int k = 0; k < p.a.arrays; ++k) {
+    tile_bytes += kMoveRows * p.a.row_bytes[k];
+    if (p.a.vec[k] == 16) bulk_row += p.a.row_bytes[k];
+  }
+  if (threadIdx.x == 0) {
+    gave_up[0] = gave_up[1] = 0;
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&full[i], 33);  // each lane's words, and the bulk copies
+      mbar_init(&empty[i], p.compact ? 2 : 1);
+    }
+    fence_barrier_init();
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    // Lane 0 has the ticket of the next round, fetched during this one.
+    auto take = [&](uint32_t t) -> uint32_t { return !p.compact ? t + gridDim.x : lane == 0 ? atomicAdd(p.ticket, 1u) : 0; };
+    uint32_t t = __shfl_sync(0xffffffffu, p.compact ? take(0) : blockIdx.x, 0), next = take(t);
+    MoveTile tile = t < total ? p.tiles[t % p.n_tiles] : MoveTile{};
+    for (int i = 0;; ++i) {
+      const int q = i % stages;
+      if (i >= stages && !mbar_wait(&empty[q], (i / stages - 1) & 1, &gave_up[0], p.err, ERR_TIMEOUT_EMPTY)) return;
+      if (lane == 0) {
+        slot[q].tile = tile;
+        slot[q].t = t;
+      }
+      if (t >= total) {  // tells the writing warp to stop
+        if (lane == 0) mbar_arrive(&full[q]);
+        mbar_arrive(&full[q]);
+        return;
+      }
+      const int pool = t / p.n_tiles;
+      uint8_t *buf = ring + (size_t)q * tile_bytes;
+      if (lane == 0) mbar_arrive_expect_tx(&full[q], tile.n * bulk_row);
+      for (int k = 0; k < p.a.arrays; ++k) {
+        const uint8_t *src = p.a.base[k][pool] + (size_t)tile.src * p.a.row_bytes[k];
+        if (p.a.vec[k] == 16) {
+          if (lane == 0) bulk_load(buf, src, tile.n * p.a.row_bytes[k], &full[q]);
+        } else if (lane < tile.n) {  // one word a row
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(buf) + 4 * lane), "l"(src + 4 * lane)
+                       : "memory");
+        }
+        buf += kMoveRows * p.a.row_bytes[k];
+      }
+      cp_async_arrive(&full[q]);
+      t = __shfl_sync(0xffffffffu, next, 0);
+      if (t < total) {
+        tile = p.tiles[t % p.n_tiles];
+        next = take(t);
+      }
+    }
+  }
+  if (threadIdx.x >= 64) {
+    // Tells of the tiles read.  Not the writing warp: the flag's release would
+    // wait for that warp's own stores first.
+    if (lane != 0) return;
+    for (int i = 0;; ++i) {
+      const int q = i % stages;
+      if (!mbar_wait(&full[q], (i / stages) & 1, &gave_up[1], p.err, ERR_TIMEOUT_FULL)) return;
+      const uint32_t t = slot[q].t;
+      if (t >= total) return;
+      set_read(p.read + t);
+      mbar_arrive(&empty[q]);
+    }
+  }
+  for (int i = 0;; ++i) {
+    const int q = i % stages;
+    if (!mbar_wait(&full[q], (i / stages) & 1, &gave_up[1], p.err, ERR_TIMEOUT_FULL)) break;
+    const uint32_t t = slot[q].t;
+    if (t >= total) break;
+    const MoveTile tile = slot[q].tile;
+    const int pool = t / p.n_tiles;
+    bool late = false;
+    if (p.compact) {
+      const uint32_t *flags = p.read + (size_t)pool * p.n_tiles + tile.dep;
+      late = lane < tile.deps && !wait_read(flags + lane);
+      late = __any_sync(0xffffffffu, late);
+      if (late && lane == 0) atomicOr(p.err, ERR_TIMEOUT_FULL);
+      asm volatile("fence.proxy.async;" ::: "memory");
+    }
+    uint8_t *buf = ring + (size_t)q * tile_bytes;
+    for (int k = 0; k < p.a.arrays && !late; ++k) {  // late: left unwritten rather than lose an unread row
+      uint8_t *dst = p.a.base[k][pool] + (size_t)tile.dst * p.a.row_bytes[k];
+      if (p.a.vec[k] == 16) {
+        if (lane == 0) bulk_store(dst, buf, tile.n * p.a.row_bytes[k]);
+      } else if (lane < tile.n) {
+        reinterpret_cast<uint32_t *>(dst)[lane] = reinterpret_cast<const uint32_t *>(buf)[lane];
+      }
+      buf += kMoveRows * p.a.row_bytes[k];
+    }
+    __syncwarp();
+    if (lane == 0) {
+      bulk_commit();
+      if (i > 0) {
+        bulk_wait_read<1>();  // the tile before has left its slot
+        mbar_arrive(&empty[(i - 1) % stages]);
+      }
+    }
+  }
+  if (lane == 0) bulk_wait<0>();
 }
 
 // Fills the arrays of the pools; checks pointers, row sizes and that no two
@@ -226,7 +375,7 @@ static int set_pools(PoolArrays &a, void *const *const arrays[3], const long lon
   int n = 0;
   for (int k = 0; k < n_arrays; ++k) {
     if (!arrays[k]) return fail("pools: null array");
-    if (row_bytes[k] < 1 || row_bytes[k] > kTileBytes) return fail("pools: rows of %lld bytes", row_bytes[k]);
+    if (row_bytes[k] < 1 || row_bytes[k] > kMaxRowBytes) return fail("pools: rows of %lld bytes", row_bytes[k]);
     a.row_bytes[k] = (int)row_bytes[k];
     uintptr_t bits = (uintptr_t)row_bytes[k] | 16;
     for (int i = 0; i < n_pools; ++i) {
@@ -313,9 +462,6 @@ KVL_EXPORT int kvl_mla_tree_accept_q8(int8_t *const *d_latent_q8, float *const *
   return accept(p, batch, d_base, d_path, d_count, max_path, d_kept, rows, static_cast<cudaStream_t>(stream));
 }
 
-// Rows of a move tile.
-static constexpr int kMoveRows = 32;
-
 KVL_EXPORT int kvl_mla_move_plan_create(KvlMlaMovePlan **plan, int runs, const int64_t *src, const int64_t *dst,
                                         const int64_t *count) {
   if (!plan) return fail("move plan: null plan");
@@ -357,10 +503,7 @@ KVL_EXPORT int kvl_mla_move_plan_create(KvlMlaMovePlan **plan, int runs, const i
     for (const Run &r : v) {
       if (r.s == r.d) continue;
       for (; k < by_src.size() && by_src[k].s < r.d + r.n; ++k) reach = std::max(reach, by_src[k].s + by_src[k].n);
-      if (reach > r.d) {  // some source that starts before this destination's end reaches into it: look closely
-        for (size_t j = 0; j < k && !overlap; ++j) overlap = by_src[j].s + by_src[j].n > r.d && by_src[j].s < r.d + r.n;
-      }
-      if (overlap) break;
+      overlap |= reach > r.d;  // a source that starts before this destination's end reaches into it
     }
     if (overlap && !(ordered && down)) {
       delete p;
@@ -373,16 +516,18 @@ KVL_EXPORT int kvl_mla_move_plan_create(KvlMlaMovePlan **plan, int runs, const i
       if (r.s == r.d) continue;
       p->moved += r.n;
       for (long long o = 0; o < r.n; o += kMoveRows)
-        p->tiles.push_back({r.s + o, r.d + o, (int)std::min<long long>(kMoveRows, r.n - o), 0});
+        p->tiles.push_back({(int)(r.s + o), (int)(r.d + o), 0, (uint16_t)std::min<long long>(kMoveRows, r.n - o), 0});
     }
     if (p->compact) {
       // sources and destinations both ascend: the tiles whose sources a
       // destination overlaps are neighbours
-      size_t lo = 0;
+      size_t lo = 0, hi = 0;
       for (size_t i = 0; i < p->tiles.size(); ++i) {
         MoveTile &t = p->tiles[i];
         while (lo < i && p->tiles[lo].src + p->tiles[lo].n <= t.dst) ++lo;
+        while (hi < i && p->tiles[hi].src < t.dst + t.n) ++hi;
         t.dep = (int)lo;
+        t.deps = (uint16_t)(std::max(lo, hi) - lo);  // at most one a row of the tile
       }
     }
     if (p->tiles.size() > (1u << 24)) {
@@ -443,17 +588,26 @@ static int move_rows(const KvlMlaMovePlan *plan, MoveParams &p, int64_t rows, cu
   const long long total = (long long)p.n_tiles * p.a.pools;
   if (total >= (1LL << 31)) return fail("pool move: too many rows");
   size_t smem = 0;
-  for (int k = 0; k < p.a.arrays; ++k) smem += ((size_t)kMoveRows * p.a.row_bytes[k] + 15) & ~size_t(15);
-  if (smem > 227 * 1024) return fail("pool move: rows of %zu bytes", smem / kMoveRows);
+  bool bulk = true;
+  for (int k = 0; k < p.a.arrays; ++k) {
+    smem += ((size_t)kMoveRows * p.a.row_bytes[k] + 15) & ~size_t(15);
+    bulk &= p.a.vec[k] == 16 || (p.a.vec[k] == 4 && p.a.row_bytes[k] == 4);
+  }
+  if (smem > kMoveSmem) return fail("pool move: rows of %zu bytes", smem / kMoveRows);
+  const size_t ring = p.compact ? kMoveSmem / 2 : kForkSmem;
+  p.stages = (int)std::min<size_t>(kMaxStages, std::max<size_t>(2, ring / smem));
+  bulk &= p.stages * smem <= kMoveSmem;
+  const int per_sm = bulk ? (p.stages * smem <= kMoveSmem / 2 ? 2 : 1)
+                          : std::max(1, std::min(6, (int)(kMoveSmem / smem)));
+  if (bulk) smem *= p.stages;
+  const auto kernel = bulk ? pool_move_kernel : pool_move_any_kernel;
   cudaError_t e = cudaSuccess;
-  if (smem > 48 * 1024)
-    e = cudaFuncSetAttribute(pool_move_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e == cudaSuccess && p.compact)
     e = cudaMemsetAsync(p.ticket, 0, 252 + (size_t)total * sizeof(uint32_t), s);
   if (e == cudaSuccess) {
     ProfScope ps("pool_move", s);
-    const int per_sm = std::max(1, std::min(6, (int)(220 * 1024 / smem)));
-    pool_move_kernel<<<(int)std::min<long long>(total, (long long)per_sm * sms), 256, smem, s>>>(p);
+    kernel<<<(int)std::min<long long>(total, (long long)per_sm * sms), bulk ? (p.compact ? 96 : 64) : 256, smem, s>>>(p);
     e = cudaGetLastError();
   }
   return e == cudaSuccess ? 0 : fail("pool move launch failed: %s", cudaGetErrorString(e));
