@@ -32,6 +32,7 @@
 #include "gemm.cuh"
 #include "mla_kernels.cuh"
 #include "peer_merge.cuh"
+#include "tree_plan.cuh"
 
 #define KVL_EXPORT extern "C" __attribute__((visibility("default")))
 
@@ -1761,13 +1762,12 @@ KVL_EXPORT size_t kvl_mla_decode_step_workspace_bytes(const KvlMlaConfig *cfg, i
 // kernels, which read each weight once per 8 tokens.
 constexpr int kStepGemmBatch = 16;
 
-static bool step_gemm_ok(const KvlMlaConfig &c, const KvlMlaDeviceWeights &w, const float *d_out, const void *ws,
-                         int batch) {
+static bool step_gemm_ok(const KvlMlaConfig &c, const KvlMlaDeviceWeights &w, const float *d_out, const void *ws) {
   const uintptr_t a = reinterpret_cast<uintptr_t>(w.q_proj) | reinterpret_cast<uintptr_t>(w.kv_a_proj) |
                       reinterpret_cast<uintptr_t>(w.kv_b_proj) | reinterpret_cast<uintptr_t>(w.o_proj) |
                       reinterpret_cast<uintptr_t>(d_out) | reinterpret_cast<uintptr_t>(ws);
   // 16-byte tensor-map bases and row strides, 16-byte vector stores
-  return batch >= kStepGemmBatch && (a & 15) == 0 && c.hidden_size % 8 == 0 && c.qk_nope_dim % 8 == 0 &&
+  return (a & 15) == 0 && c.hidden_size % 8 == 0 && c.qk_nope_dim % 8 == 0 &&
          c.qk_rope_dim % 8 == 0 && c.kv_lora_rank % 8 == 0 && c.v_head_dim % 8 == 0;
 }
 
@@ -1814,14 +1814,34 @@ static int step_attend(const KvlMlaAttendPlan *plan, const StepPool &pool, const
   return attend_common(plan, a, cfg.num_heads, cfg.kv_lora_rank, cfg.qk_rope_dim, s);
 }
 
-// Tensor-core projections of one decode step (batch >= kStepGemmBatch).
-static int decode_step_gemm(const KvlMlaConfig &cfg, const KvlMlaDeviceWeights &w, const KvlMlaAttendPlan *plan,
+// The attend of a step on the tensor cores: one token a sequence over `plan`
+// (fp32 queries and outputs), or the nodes of drafted trees (bf16 ones).
+struct StepAttend {
+  const KvlMlaAttendPlan *plan = nullptr;
+  const KvlMlaTreePlan *tree = nullptr;
+  const uint64_t *mask = nullptr;
+  uint32_t *err() const { return tree ? static_cast<uint32_t *>(tree->d_meta) : plan->dp.err_word(); }
+};
+
+static int step_attend_tree(const StepAttend &at, const StepPool &pool, const KvlMlaConfig &cfg, uint16_t *mix,
+                            const uint16_t *qabs, int64_t rows, cudaStream_t s) {
+  const float scale = 1.0f / sqrtf(static_cast<float>(cfg.qk_nope_dim + cfg.qk_rope_dim));
+  const int NH = cfg.num_heads, R = cfg.kv_lora_rank, DR = cfg.qk_rope_dim;
+  return pool.q8() ? kvl_mla_tree_attend_q8(at.tree, mix, nullptr, qabs, at.mask, pool.lat8, pool.lscale, pool.rope16,
+                                            rows, NH, R, DR, scale, s)
+                   : kvl_mla_tree_attend_bf16(at.tree, mix, nullptr, qabs, at.mask, pool.kv, rows, NH, R, DR, scale, s);
+}
+
+// Tensor-core projections of one decode step (batch >= kStepGemmBatch), or of
+// the verification of drafted trees (any number of nodes).
+static int decode_step_gemm(const KvlMlaConfig &cfg, const KvlMlaDeviceWeights &w, const StepAttend &at,
                             float *d_out, const float *d_x, const StepPool &pool, int64_t rows, const int64_t *d_row,
                             const int *d_pos, int B, uint8_t *ws, const size_t *off, cudaStream_t s) {
   const uint64_t H = cfg.hidden_size, NH = cfg.num_heads, DN = cfg.qk_nope_dim, DR = cfg.qk_rope_dim;
   const uint64_t DV = cfg.v_head_dim, R = cfg.kv_lora_rank, QD = DN + DR, b = B;
   float *q = reinterpret_cast<float *>(ws + off[0]);
   float *qabs = reinterpret_cast<float *>(ws + off[2]);
+  uint16_t *qabs16 = reinterpret_cast<uint16_t *>(ws + off[2]);  // of a tree's nodes
   float *mix = reinterpret_cast<float *>(ws + off[3]);
   uint16_t *hob = reinterpret_cast<uint16_t *>(ws + off[4]);
   uint16_t *xb = reinterpret_cast<uint16_t *>(ws + off[5]);
@@ -1836,8 +1856,8 @@ static int decode_step_gemm(const KvlMlaConfig &cfg, const KvlMlaDeviceWeights &
   CK(bf16_rne(xb, d_x, static_cast<long long>(b * H), s));
   GemmParams g;
   memset(&g, 0, sizeof g);
-  g.err = plan->dp.err_word();  // a bounded wait that ran out: reported by kvl_mla_attend_check
-  g.prefetch_b = 1;             // every B operand of the step is a weight
+  g.err = at.err();  // a bounded wait that ran out: reported by kvl_mla_attend_check or kvl_mla_tree_check
+  g.prefetch_b = 1;  // every B operand of the step is a weight
   // q = x Wq^T fp32 [B][NH*QD]; ka = x Wkva^T fp32 [B][R+DR]
   if (!bf16_map(&g.tm_a, xb, H, b, H * 2, 128) || !bf16_map(&g.tm_b, w.q_proj, H, NH * QD, H * 2, 256)) {
     set_err("decode step: tensor map (q_proj)");
@@ -1867,8 +1887,12 @@ static int decode_step_gemm(const KvlMlaConfig &cfg, const KvlMlaDeviceWeights &
   CK(step_append(pool, cfg, w.kv_a_norm, ka_parts, B, d_row, d_pos, g.ksplit, g.c_bstride, s));
   g.ksplit = 0;
   g.c_bstride = 0;
-  CK(q_split(qn, qabs, q, q_parts, static_cast<long long>(b * NH * QD), B, static_cast<int>(NH),
-             static_cast<int>(DN), static_cast<int>(DR), static_cast<int>(R), cfg.rope_theta, d_pos, s));
+  if (at.tree)
+    CK(q_split(qn, qabs16, q, q_parts, static_cast<long long>(b * NH * QD), B, static_cast<int>(NH),
+               static_cast<int>(DN), static_cast<int>(DR), static_cast<int>(R), cfg.rope_theta, d_pos, s));
+  else
+    CK(q_split(qn, qabs, q, q_parts, static_cast<long long>(b * NH * QD), B, static_cast<int>(NH),
+               static_cast<int>(DN), static_cast<int>(DR), static_cast<int>(R), cfg.rope_theta, d_pos, s));
   // qabs[:, h, :R] = q_nope[:, h] . W_UK[h]   (NH products, M = B, N = R, K = DN);
   // W_UK[h] ([DN][R], rows h (DN + DV) + d of kv_b_proj) is read in place as
   // an MN-major B operand
@@ -1885,20 +1909,23 @@ static int decode_step_gemm(const KvlMlaConfig &cfg, const KvlMlaDeviceWeights &
   }
   g.N = static_cast<int>(R);
   g.K = static_cast<int>(DN);
-  g.c = qabs;
+  g.c = ws + off[2];  // qabs, or qabs16
   g.ldc = static_cast<int>(NH * (R + DR));
   g.batch = static_cast<int>(NH);
   g.c_bstride = static_cast<long long>(R + DR);
   g.b_mn = 1;
-  CK(launch_gemm(g, 256, EPI_F32, sms, s, "gemm_absorb", true));
+  CK(launch_gemm(g, 256, at.tree ? EPI_BF16 : EPI_F32, sms, s, "gemm_absorb", true));
   g.b_mn = 0;
 
-  if (step_attend(plan, pool, cfg, mix, qabs, rows, s) != 0) return -1;
-
   // ho[:, h, :] = mix[:, h] . W_UV[h]^T   (NH products, M = B, N = DV, K = R), bf16
-  CK(mix_heads_bf16(mixb, mix, B, static_cast<int>(NH), static_cast<int>(R), s));
+  if (at.tree) {  // mix is bf16 already, [B][NH][R]
+    if (step_attend_tree(at, pool, cfg, mixb, qabs16, rows, s) != 0) return -1;
+  } else {
+    if (step_attend(at.plan, pool, cfg, mix, qabs, rows, s) != 0) return -1;
+    CK(mix_heads_bf16(mixb, mix, B, static_cast<int>(NH), static_cast<int>(R), s));
+  }
   {
-    const uint64_t ad[3] = {R, b, NH}, as[2] = {R * 2, b * R * 2};
+    const uint64_t ad[3] = {R, b, NH}, as[2] = {(at.tree ? NH * R : R) * 2, (at.tree ? R : b * R) * 2};
     const uint64_t bd[3] = {R, DV, NH}, bs[2] = {R * 2, (DN + DV) * R * 2};
     const uint32_t abox[3] = {64, 128, 1}, bbox[3] = {64, 128, 1};
     if (!make_tmap_3d(&g.tm_a, mixb, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ad, as, abox, CU_TENSOR_MAP_SWIZZLE_128B) ||
@@ -1945,8 +1972,11 @@ static int decode_step(const KvlMlaConfig *cfg, const KvlMlaDeviceWeights *w, co
   size_t off[12];
   step_ws_layout(*cfg, batch, off);
   uint8_t *ws = static_cast<uint8_t *>(d_workspace);
-  if (step_gemm_ok(*cfg, *w, d_out, ws, batch))
-    return decode_step_gemm(*cfg, *w, plan, d_out, d_x, pool, rows, d_row, d_pos, batch, ws, off, s);
+  if (batch >= kStepGemmBatch && step_gemm_ok(*cfg, *w, d_out, ws)) {
+    StepAttend at;
+    at.plan = plan;
+    return decode_step_gemm(*cfg, *w, at, d_out, d_x, pool, rows, d_row, d_pos, batch, ws, off, s);
+  }
   float *q = reinterpret_cast<float *>(ws + off[0]);
   float *ka = reinterpret_cast<float *>(ws + off[1]);
   float *qabs = reinterpret_cast<float *>(ws + off[2]);
@@ -1993,6 +2023,78 @@ KVL_EXPORT int kvl_mla_decode_step_q8(const KvlMlaConfig *cfg, const KvlMlaDevic
   pool.lscale = d_latent_scale;
   pool.rope16 = d_rope_bf16;
   return decode_step(cfg, w, plan, d_out, d_x, pool, rows, d_row, d_pos, batch, d_workspace, stream);
+}
+
+// The step for drafted trees: every node's row is appended where the plan has
+// it, then all nodes attend.
+static int tree_step(const KvlMlaConfig *cfg, const KvlMlaDeviceWeights *w, const KvlMlaTreePlan *plan, float *d_out,
+                     const float *d_x, const uint64_t *d_mask, const int *d_pos, const StepPool &pool, int64_t rows,
+                     void *d_workspace, void *stream) {
+  if (!cfg || !w || !plan || !d_out || !d_x || !d_mask || !d_pos || !d_workspace || !cfg_dims_ok(*cfg) ||
+      !w->q_proj || !w->kv_a_proj || !w->kv_a_norm || !w->kv_b_proj || !w->o_proj) {
+    set_err("invalid tree step arguments");
+    return -1;
+  }
+  if (cfg->num_heads != plan->nh || cfg->kv_lora_rank != plan->R) {
+    set_err("tree step: the plan is for %d heads x %d", plan->nh, plan->R);
+    return -1;
+  }
+  if (rows < plan->host.rows_needed) {  // before anything is appended
+    set_err("tree step: a sequence ends at pool row %lld, the pool has %lld", plan->host.rows_needed,
+            static_cast<long long>(rows));
+    return -1;
+  }
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev != plan->device) {
+    set_err("tree step: the plan belongs to device %d, the current device is %d", plan->device, dev);
+    return -1;
+  }
+  const uintptr_t wide = reinterpret_cast<uintptr_t>(pool.kv) | reinterpret_cast<uintptr_t>(pool.lat8) |
+                         reinterpret_cast<uintptr_t>(pool.rope16);
+  if (!step_gemm_ok(*cfg, *w, d_out, d_workspace) || cfg->qk_rope_dim > 256 || (wide & 15) ||
+      ((reinterpret_cast<uintptr_t>(d_x) | reinterpret_cast<uintptr_t>(d_pos) |
+        reinterpret_cast<uintptr_t>(pool.lscale)) & 3) ||
+      (reinterpret_cast<uintptr_t>(d_mask) & 7)) {
+    set_err("tree step: weights, output, workspace and pool must be 16-byte aligned and every width a multiple of 8");
+    return -1;
+  }
+  const int nodes = plan->host.nodes;
+  size_t off[12];
+  step_ws_layout(*cfg, nodes, off);
+  StepAttend at;
+  at.tree = plan;
+  at.mask = d_mask;
+  const int64_t *d_row = reinterpret_cast<const int64_t *>(static_cast<const uint8_t *>(plan->d_meta) + plan->off_rows);
+  return decode_step_gemm(*cfg, *w, at, d_out, d_x, pool, rows, d_row, d_pos, nodes, static_cast<uint8_t *>(d_workspace),
+                          off, static_cast<cudaStream_t>(stream));
+}
+
+KVL_EXPORT int kvl_mla_tree_step_bf16(const KvlMlaConfig *cfg, const KvlMlaDeviceWeights *w,
+                                      const KvlMlaTreePlan *plan, float *d_out, const float *d_x,
+                                      const uint64_t *d_mask, const int *d_pos, uint16_t *d_kv, int64_t rows,
+                                      void *d_workspace, void *stream) {
+  if (!d_kv) {
+    set_err("tree step: null kv pool");
+    return -1;
+  }
+  StepPool pool;
+  pool.kv = d_kv;
+  return tree_step(cfg, w, plan, d_out, d_x, d_mask, d_pos, pool, rows, d_workspace, stream);
+}
+
+KVL_EXPORT int kvl_mla_tree_step_q8(const KvlMlaConfig *cfg, const KvlMlaDeviceWeights *w, const KvlMlaTreePlan *plan,
+                                    float *d_out, const float *d_x, const uint64_t *d_mask, const int *d_pos,
+                                    int8_t *d_latent_q8, float *d_latent_scale, uint16_t *d_rope_bf16, int64_t rows,
+                                    void *d_workspace, void *stream) {
+  if (!d_latent_q8 || !d_latent_scale || !d_rope_bf16) {
+    set_err("tree step: null q8 pool");
+    return -1;
+  }
+  StepPool pool;
+  pool.lat8 = d_latent_q8;
+  pool.lscale = d_latent_scale;
+  pool.rope16 = d_rope_bf16;
+  return tree_step(cfg, w, plan, d_out, d_x, d_mask, d_pos, pool, rows, d_workspace, stream);
 }
 
 KVL_EXPORT int kvl_mla_merge_packed(float *d_out, float *d_lse, const float *d_parts, int parts, int batch,

@@ -681,7 +681,11 @@ cudaError_t vup(float *ho, const float *mix, const uint16_t *kvb, int n, int NH,
 // once), then one rope pair per thread; cos/sin once per block.
 constexpr int kQsHeads = 4;
 
-__global__ void __launch_bounds__(128) q_split_kernel(uint16_t *qn, float *qabs, const float *q, int parts,
+__device__ __forceinline__ void put(float *p, float v) { *p = v; }
+__device__ __forceinline__ void put(uint16_t *p, float v) { *p = __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
+
+template <typename QT>
+__global__ void __launch_bounds__(128) q_split_kernel(uint16_t *qn, QT *qabs, const float *q, int parts,
                                                       long long part_stride, int n, int NH, int DN, int DR, int R,
                                                       float theta, const int *pos_of) {
   __shared__ float2 cs[128];
@@ -734,19 +738,30 @@ __global__ void __launch_bounds__(128) q_split_kernel(uint16_t *qn, float *qabs,
     }
     float lo, hi;
     rope_rotate(a, b, cs[i].x, cs[i].y, lo, hi);
-    float *dst = qabs + (static_cast<size_t>(t) * NH + h) * (R + DR);
-    dst[R + i] = lo;
-    dst[R + half + i] = hi;
+    QT *dst = qabs + (static_cast<size_t>(t) * NH + h) * (R + DR);
+    put(dst + R + i, lo);
+    put(dst + R + half + i, hi);
   }
+}
+
+template <typename QT>
+static cudaError_t launch_q_split(uint16_t *qn, QT *qabs, const float *q, int parts, long long part_stride, int n,
+                                  int NH, int DN, int DR, int R, float theta, const int *pos_of, cudaStream_t s) {
+  if (n <= 0) return cudaSuccess;
+  if (DR / 2 > 128) return cudaErrorInvalidValue;
+  ProfScope ps("q_split", s);
+  return launch_dependent(q_split_kernel<QT>, dim3(n, (NH + kQsHeads - 1) / kQsHeads), dim3(128), 0, s, qn, qabs, q,
+                          parts, part_stride, n, NH, DN, DR, R, theta, pos_of);
 }
 
 cudaError_t q_split(uint16_t *qn, float *qabs, const float *q, int parts, long long part_stride, int n, int NH,
                     int DN, int DR, int R, float theta, const int *pos_of, cudaStream_t s) {
-  if (n <= 0) return cudaSuccess;
-  if (DR / 2 > 128) return cudaErrorInvalidValue;
-  ProfScope ps("q_split", s);
-  return launch_dependent(q_split_kernel, dim3(n, (NH + kQsHeads - 1) / kQsHeads), dim3(128), 0, s, qn, qabs, q, parts,
-                          part_stride, n, NH, DN, DR, R, theta, pos_of);
+  return launch_q_split(qn, qabs, q, parts, part_stride, n, NH, DN, DR, R, theta, pos_of, s);
+}
+
+cudaError_t q_split(uint16_t *qn, uint16_t *qabs, const float *q, int parts, long long part_stride, int n, int NH,
+                    int DN, int DR, int R, float theta, const int *pos_of, cudaStream_t s) {
+  return launch_q_split(qn, qabs, q, parts, part_stride, n, NH, DN, DR, R, theta, pos_of, s);
 }
 
 // dst[i] = src[i] + src[stride + i] + ... (parts terms, in order), fp32.

@@ -34,6 +34,9 @@ cudaError_t vup(float *ho, const float *mix, const uint16_t *kvb, int n, int NH,
                 cudaStream_t s);
 cudaError_t q_split(uint16_t *qn, float *qabs, const float *q, int parts, long long part_stride, int n, int NH,
                     int DN, int DR, int R, float theta, const int *pos_of, cudaStream_t s);
+// The same with a bf16 absorbed query (its rope part rounded to nearest).
+cudaError_t q_split(uint16_t *qn, uint16_t *qabs, const float *q, int parts, long long part_stride, int n, int NH,
+                    int DN, int DR, int R, float theta, const int *pos_of, cudaStream_t s);
 cudaError_t sum_parts(float *dst, const float *src, int parts, long long stride, long long n, cudaStream_t s);
 cudaError_t mix_heads_bf16(uint16_t *out, const float *mix, int n, int NH, int R, cudaStream_t s);
 cudaError_t quantize_rows(int8_t *q, float *scale, const float *x, int rows, int R, cudaStream_t s);

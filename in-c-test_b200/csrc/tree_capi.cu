@@ -32,6 +32,10 @@ static int fail(const char *fmt, ...) {
 // The plan's arrays in one device allocation, the partials in another.
 static int upload(KvlMlaTreePlan &p) {
   const TreeHostPlan &h = p.host;
+  std::vector<long long> rows;  // of the nodes in the pool
+  rows.reserve(h.nodes);
+  for (size_t b = 0; b < h.row0.size(); ++b)
+    for (int j = 0; j < h.tree[b]; ++j) rows.push_back(h.row0[b] + h.len[b] + j);
   struct Part {
     const void *src;
     size_t bytes;
@@ -44,6 +48,7 @@ static int upload(KvlMlaTreePlan &p) {
       {h.tree.data(), h.tree.size() * sizeof(int), &p.off_tree},
       {h.first_node.data(), h.first_node.size() * sizeof(int), &p.off_first},
       {h.seq_of_node.data(), h.seq_of_node.size() * sizeof(int), &p.off_seq},
+      {rows.data(), rows.size() * sizeof(long long), &p.off_rows},
   };
   size_t at = 256;  // the error word
   for (Part &q : parts) {

@@ -10,5 +10,5 @@ struct KvlMlaTreePlan {
   void *d_meta = nullptr;  // error word, then the arrays below
   void *d_work = nullptr;  // partial outputs and lse values
   size_t off_items = 0, off_merge = 0, off_row0 = 0, off_len = 0, off_tree = 0, off_first = 0,
-         off_seq = 0;
+         off_seq = 0, off_rows = 0;
 };

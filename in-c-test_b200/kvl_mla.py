@@ -122,6 +122,10 @@ SIGNATURES = {
                                                               C.c_void_p]),
     "kvl_mla_tree_attend_q8": (C.c_int, [C.c_void_p] * 8 + [C.c_int64, C.c_int, C.c_int, C.c_int, C.c_float,
                                                             C.c_void_p]),
+    "kvl_mla_tree_step_bf16": (C.c_int, [C.POINTER(KvlMlaConfig), C.POINTER(KvlMlaDeviceWeights)] + [C.c_void_p] * 6 + [
+        C.c_int64, C.c_void_p, C.c_void_p]),
+    "kvl_mla_tree_step_q8": (C.c_int, [C.POINTER(KvlMlaConfig), C.POINTER(KvlMlaDeviceWeights)] + [C.c_void_p] * 8 + [
+        C.c_int64, C.c_void_p, C.c_void_p]),
     "kvl_mla_tree_check": (C.c_int, [C.c_void_p, C.c_void_p]),
     "kvl_mla_tree_accept_bf16": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_void_p,
                                            C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),
@@ -394,6 +398,17 @@ class TreePlan:
         check(self.lib.kvl_mla_tree_attend_q8(self.h, t_ptr(out), t_ptr(lse), t_ptr(q), t_ptr(mask), t_ptr(lat8),
                                               t_ptr(lscale), t_ptr(rope16), rows, self.num_heads, self.kv_lora_rank,
                                               rope_dim, float(scale), stream), "tree attend")
+
+    def step_bf16(self, cfg, weights, out, x, mask, pos, kv, rows, workspace, stream=0):
+        """kvl_mla_tree_step_bf16: cfg a KvlMlaConfig, weights a KvlMlaDeviceWeights, workspace of
+        kvl_mla_decode_step_workspace_bytes(cfg, nodes) bytes."""
+        check(self.lib.kvl_mla_tree_step_bf16(C.byref(cfg), C.byref(weights), self.h, t_ptr(out), t_ptr(x), t_ptr(mask),
+                                              t_ptr(pos), t_ptr(kv), rows, t_ptr(workspace), stream), "tree step")
+
+    def step_q8(self, cfg, weights, out, x, mask, pos, lat8, lscale, rope16, rows, workspace, stream=0):
+        check(self.lib.kvl_mla_tree_step_q8(C.byref(cfg), C.byref(weights), self.h, t_ptr(out), t_ptr(x), t_ptr(mask),
+                                            t_ptr(pos), t_ptr(lat8), t_ptr(lscale), t_ptr(rope16), rows,
+                                            t_ptr(workspace), stream), "tree step")
 
     def check(self, stream=0):
         return self.lib.kvl_mla_tree_check(self.h, stream)

@@ -257,6 +257,24 @@ int kvl_mla_tree_attend_q8(const KvlMlaTreePlan *plan, uint16_t *d_out, float *d
                            const uint64_t *d_mask, const int8_t *d_latent_q8, const float *d_latent_scale,
                            const uint16_t *d_rope_bf16, int64_t rows, int num_heads, int kv_lora_rank, int rope_dim,
                            float softmax_scale, void *stream);
+/* One layer's step for drafted trees, the decode step of the section above with
+ * the plan's nodes in place of one token a sequence: projections of all nodes'
+ * activations, append of each node's row where the plan has it (behind its
+ * sequence's cache; RoPE position d_pos[node], the cached length plus the
+ * node's depth), attend under d_mask, V up-projection and o_proj.  d_x/d_out
+ * [nodes][H] fp32, d_pos [nodes].  The projections run as tensor-core GEMMs on
+ * bf16-rounded activations for any number of nodes: weights, d_out, workspace
+ * and pool 16-byte aligned, every width a multiple of 8, else -1 before
+ * anything is launched.  Workspace of
+ * kvl_mla_decode_step_workspace_bytes(cfg, nodes).  Device-side errors are
+ * reported by kvl_mla_tree_check. */
+int kvl_mla_tree_step_bf16(const KvlMlaConfig *cfg, const KvlMlaDeviceWeights *w, const KvlMlaTreePlan *plan,
+                           float *d_out, const float *d_x, const uint64_t *d_mask, const int *d_pos, uint16_t *d_kv,
+                           int64_t rows, void *d_workspace, void *stream);
+int kvl_mla_tree_step_q8(const KvlMlaConfig *cfg, const KvlMlaDeviceWeights *w, const KvlMlaTreePlan *plan,
+                         float *d_out, const float *d_x, const uint64_t *d_mask, const int *d_pos,
+                         int8_t *d_latent_q8, float *d_latent_scale, uint16_t *d_rope_bf16, int64_t rows,
+                         void *d_workspace, void *stream);
 /* Waits for `stream` and returns -1 if a kernel of the plan's calls reported a
  * device-side error (a bounded wait that ran out); clears it. */
 int kvl_mla_tree_check(const KvlMlaTreePlan *plan, void *stream);
