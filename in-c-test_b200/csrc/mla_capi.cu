@@ -2052,6 +2052,10 @@ static int tree_step(const KvlMlaConfig *cfg, const KvlMlaDeviceWeights *w, cons
             static_cast<long long>(rows));
     return -1;
   }
+  if (!plan->host.own_rows) {
+    set_err("tree step: two sequences of the plan have the same drafted row");
+    return -1;
+  }
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess || dev != plan->device) {
     set_err("tree step: the plan belongs to device %d, the current device is %d", plan->device, dev);

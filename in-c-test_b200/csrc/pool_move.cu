@@ -419,6 +419,13 @@ static int accept(AcceptParams &p, int batch, const int64_t *base, const int *pa
   if ((reinterpret_cast<uintptr_t>(base) & 7) ||
       ((reinterpret_cast<uintptr_t>(path) | reinterpret_cast<uintptr_t>(count) | reinterpret_cast<uintptr_t>(kept)) & 3))
     return fail("tree accept: a pointer is not aligned to its type");
+  // the blocks of all pools read the inputs while one of them writes `kept`
+  auto meets = [&](const void *x, size_t bytes) {
+    const uintptr_t k = reinterpret_cast<uintptr_t>(kept), i = reinterpret_cast<uintptr_t>(x);
+    return kept && k < i + bytes && i < k + 4 * (size_t)batch;
+  };
+  if (meets(base, 8 * (size_t)batch) || meets(path, 4 * (size_t)batch * max_path) || meets(count, 4 * (size_t)batch))
+    return fail("tree accept: d_kept overlaps an input");
   p.base = base;
   p.path = path;
   p.count = count;

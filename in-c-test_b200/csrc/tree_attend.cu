@@ -38,6 +38,12 @@ int build_tree_plan(TreeHostPlan &hp, int batch, const int *cached_len, const in
     hp.nodes += nodes[b];
   }
   if (hp.nodes == 0) return -1;
+  std::vector<std::pair<long long, int>> drafted;
+  for (int b = 0; b < batch; ++b)
+    if (nodes[b]) drafted.push_back({row0[b] + cached_len[b], nodes[b]});
+  std::sort(drafted.begin(), drafted.end());
+  for (size_t i = 1; i < drafted.size(); ++i)
+    hp.own_rows &= drafted[i - 1].first + drafted[i - 1].second <= drafted[i].first;
 
   struct Seq {
     int tiles, groups;

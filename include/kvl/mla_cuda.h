@@ -247,7 +247,7 @@ int kvl_mla_tree_mask(uint64_t *mask, const int *parent, int nodes);
  * used.  Scores, softmax sums and the accumulation are fp32; the softmax
  * weights enter the P.V product as bf16.  The production shape (16, 512, 64)
  * runs on the tensor cores and wants d_q, d_out and the pool's arrays 16-byte
- * aligned; other shapes run a CUDA-core kernel.  A device-side error is
+ * aligned; other shapes run a CUDA-core kernel.  The outputs overlap no input.  A device-side error is
  * reported by kvl_mla_tree_check. */
 int kvl_mla_tree_attend_bf16(const KvlMlaTreePlan *plan, uint16_t *d_out, float *d_lse, const uint16_t *d_q,
                              const uint64_t *d_mask, const uint16_t *d_kv, int64_t rows, int num_heads,
@@ -265,7 +265,8 @@ int kvl_mla_tree_attend_q8(const KvlMlaTreePlan *plan, uint16_t *d_out, float *d
  * [nodes][H] fp32, d_pos [nodes].  The projections run as tensor-core GEMMs on
  * bf16-rounded activations for any number of nodes: weights, d_out, workspace
  * and pool 16-byte aligned, every width a multiple of 8, else -1 before
- * anything is launched.  Workspace of
+ * anything is launched.  Sequences may share cached rows, drafted rows that two
+ * of them share are refused.  Workspace of
  * kvl_mla_decode_step_workspace_bytes(cfg, nodes).  Device-side errors are
  * reported by kvl_mla_tree_check. */
 int kvl_mla_tree_step_bf16(const KvlMlaConfig *cfg, const KvlMlaDeviceWeights *w, const KvlMlaTreePlan *plan,
@@ -284,7 +285,7 @@ int kvl_mla_tree_check(const KvlMlaTreePlan *plan, void *stream);
  * node 0; a path ascends, as parents come before their children), in each of
  * n_pools pools (1 to 64, e.g. one per layer) of `rows` rows; other rows stay
  * as they are.  d_path is [batch][max_path], max_path at most 64.  d_kept
- * [batch] (may be NULL) receives d_count[b], or -1 where nothing was moved
+ * [batch] (may be NULL; overlaps no input) receives d_count[b], or -1 where nothing was moved
  * because the path does not ascend, leaves the pool, or shares rows with
  * another sequence of the call.  pools: host array of device pointers. */
 int kvl_mla_tree_accept_bf16(uint16_t *const *d_pools, int n_pools, int64_t rows, int kv_lora_rank, int rope_dim,
@@ -303,7 +304,8 @@ int kvl_mla_tree_accept_q8(int8_t *const *d_latent_q8, float *const *d_latent_sc
  * slide together after others ended).  Every destination row receives what its
  * source row held before the call.  Two runs that write one row, and other
  * overlaps, are refused.  Created on and used with the current device; calls of
- * one plan must be ordered by their streams. */
+ * one plan must be ordered by their streams, those of captured graphs included,
+ * which must not outlive the plan. */
 typedef struct KvlMlaMovePlan KvlMlaMovePlan;
 
 int kvl_mla_move_plan_create(KvlMlaMovePlan **plan, int runs, const int64_t *src, const int64_t *dst,

@@ -79,5 +79,7 @@ def test_null_arguments_of_moves(K):
                  (one, 1, 10, 0, 64, 1, 8, 8, 8, 4, None, None), (one, 1, 10, 512, 64, 0, 8, 8, 8, 4, None, None),
                  (one, 1, 10, 512, 64, 1, None, 8, 8, 4, None, None), (one, 1, 10, 512, 64, 1, 8, None, 8, 4, None, None),
                  (one, 1, 10, 512, 64, 1, 8, 8, None, 4, None, None), (one, 1, 10, 512, 64, 1, 8, 8, 8, 0, None, None),
-                 (one, 1, 10, 512, 64, 1, 8, 8, 8, 65, None, None), (one, 1, 10, 512, 64, 1, 4, 8, 8, 4, None, None)]:
+                 (one, 1, 10, 512, 64, 1, 8, 8, 8, 65, None, None), (one, 1, 10, 512, 64, 1, 4, 8, 8, 4, None, None),
+                 (one, 1, 10, 512, 64, 1, 8, 64, 96, 4, 96, None), (one, 1, 10, 512, 64, 1, 8, 64, 96, 4, 12, None),
+                 (one, 1, 10, 512, 64, 1, 8, 64, 96, 4, 76, None)]:
         assert fn(*args) == -1, args

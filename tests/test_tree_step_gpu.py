@@ -302,6 +302,9 @@ def test_step_refusals(K, torch_cuda):
         tree_step(m, pool, 0, plan, x, mask, pos, ws=m.workspace(5)[4:])
     with pytest.raises(K.KvlError, match="the plan is for 8 heads"):
         tree_step(m, pool, 0, K.TreePlan(lens, nodes, row0, num_heads=8), x, mask, pos)
+    twice = K.TreePlan([40, 38], [2, 4], [row0[0], row0[0]])
+    with pytest.raises(K.KvlError, match="the same drafted row"):
+        tree_step(m, pool, 0, twice, torch.zeros(6, H, device="cuda"), mask, pos)
     with pytest.raises(K.KvlError, match="arguments"):
         tree_step(m, pool, 0, plan, x, None, pos)
     torch.cuda.synchronize()
