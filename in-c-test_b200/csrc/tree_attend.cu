@@ -1080,7 +1080,7 @@ cudaError_t launch_tree_attend(const TreeParams &p, bool q8, int grid, cudaStrea
 // query row, as the attend's lane left them, and the parts z, z + Z, ...; the Z
 // sums are added in order.  Bound by the latency of its two passes over a few
 // parts a thread (lse, then outputs); the outputs lie in L2 mostly.
-template <int Z, int LANES, int UNROLL>
+template <int Z, int LANES, int BATCH>
 __global__ void __launch_bounds__(LANES * Z) tree_merge_kernel(uint16_t *out, float *lse, const float *part_o,
                                                                const float *part_lse, const TreeMerge *entries) {
   const TreeMerge e = entries[blockIdx.x];
@@ -1094,11 +1094,30 @@ __global__ void __launch_bounds__(LANES * Z) tree_merge_kernel(uint16_t *out, fl
   const bool real = row < e.nn * kHeads;
   const float *ls = part_lse + static_cast<size_t>(e.first) * kTreeRows + row;
   const float4 *os = reinterpret_cast<const float4 *>(part_o) + (static_cast<size_t>(e.first) * 64 + quad) * 128 + at;
+  // The loads of BATCH parts are on their way at once, the first batch's outputs
+  // before its weights are known.
+  float w[BATCH];
+  float4 v[BATCH];
+  auto load_lse = [&](int q0) {
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+      w[i] = real && q0 + Z * i < e.count ? ls[(q0 + Z * i) * kTreeRows] : -INFINITY;
+  };
+  auto load_out = [&](int q0) {
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i)
+      v[i] = real && q0 + Z * i < e.count ? os[static_cast<size_t>(q0 + Z * i) * 64 * 128] : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
   float m = -INFINITY;
-  if (real) {
-#pragma unroll UNROLL
-    for (int q = z; q < e.count; q += Z) m = fmaxf(m, ls[q * kTreeRows]);
+  for (int q0 = z + Z * BATCH; q0 < e.count; q0 += Z * BATCH) {
+    load_lse(q0);
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) m = fmaxf(m, w[i]);
   }
+  load_lse(z);
+  load_out(z);
+#pragma unroll
+  for (int i = 0; i < BATCH; ++i) m = fmaxf(m, w[i]);
   if (Z > 1) {
     max_z[z][tid] = m;
     __syncthreads();
@@ -1108,17 +1127,20 @@ __global__ void __launch_bounds__(LANES * Z) tree_merge_kernel(uint16_t *out, fl
   const float ref = m == -INFINITY ? 0.f : m;  // no part has seen a row: all weights are 0
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
-  if (real) {
-#pragma unroll UNROLL
-    for (int q = z; q < e.count; q += Z) {
-      const float w = __expf(ls[q * kTreeRows] - ref);
-      const float4 v = os[static_cast<size_t>(q) * 64 * 128];
-      sum += w;
-      acc.x = fmaf(w, v.x, acc.x);
-      acc.y = fmaf(w, v.y, acc.y);
-      acc.z = fmaf(w, v.z, acc.z);
-      acc.w = fmaf(w, v.w, acc.w);
+  for (int q0 = z;;) {
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const float wi = __expf(w[i] - ref);
+      sum += wi;
+      acc.x = fmaf(wi, v[i].x, acc.x);
+      acc.y = fmaf(wi, v[i].y, acc.y);
+      acc.z = fmaf(wi, v[i].z, acc.z);
+      acc.w = fmaf(wi, v[i].w, acc.w);
     }
+    q0 += Z * BATCH;
+    if (q0 >= e.count) break;
+    load_lse(q0);
+    load_out(q0);
   }
   if (Z > 1) {
     acc_z[z][tid] = acc;
@@ -1153,7 +1175,7 @@ cudaError_t launch_tree_merge(const TreeParams &p, const TreeMerge *entries, int
   // a few parts a thread: more threads share an entry that has many
   if (max_count <= 8) return launch(tree_merge_kernel<1, 128, 8>, 1, 128);
   if (max_count <= 32) return launch(tree_merge_kernel<4, 128, 8>, 4, 128);
-  return launch(tree_merge_kernel<16, 64, 4>, 16, 64);
+  return launch(tree_merge_kernel<16, 32, 10>, 16, 32);
 }
 
 }  // namespace kvl

@@ -314,7 +314,8 @@ void kvl_mla_move_plan_destroy(KvlMlaMovePlan *plan);
 /* compaction: whether rows that are read are written too; moved_rows: rows that
  * change their place (runs with dst == src are left out). */
 int kvl_mla_move_plan_info(const KvlMlaMovePlan *plan, int *compaction, int64_t *moved_rows);
-/* The plan's moves in each of n_pools pools (1 to 64) of `rows` rows. */
+/* The plan's moves in each of n_pools pools (1 to 64) of `rows` rows of at most
+ * 7040 bytes (of all arrays together). */
 int kvl_mla_pool_move_bf16(const KvlMlaMovePlan *plan, uint16_t *const *d_pools, int n_pools, int64_t rows,
                            int kv_lora_rank, int rope_dim, void *stream);
 int kvl_mla_pool_move_q8(const KvlMlaMovePlan *plan, int8_t *const *d_latent_q8, float *const *d_latent_scale,

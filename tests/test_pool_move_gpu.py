@@ -170,3 +170,31 @@ def test_pools_that_are_refused(K, torch_cuda):
         K.PoolSet.bf16([a[0][:, :500]])
     before = a.clone()
     assert torch.equal(a, before)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "q8"])
+@pytest.mark.parametrize("R,DR", [(1024, 64), (2000, 64), (512, 60), (16, 8), (3000, 8)])
+@pytest.mark.parametrize("src,dst,count", [([3], [0], [700]), ([0, 50], [400, 600], [133, 90])])
+def test_move_row_widths(K, torch_cuda, kind, R, DR, src, dst, count):
+    """Rows that two, one or no ring of bulk copies holds, and rows that bulk copies cannot take."""
+    a, ps = pools(K, kind, 2, 710, R, DR, seed=5)
+    plan = K.PoolMovePlan(src, dst, count)
+    want = moved(a, *runs_to_rows(src, dst, count))
+    plan.move(ps)
+    assert plan.check() == 0 and same(a, want)
+
+
+@pytest.mark.parametrize("off", [1, 2, 4, 8])
+def test_move_misaligned_pools(K, torch_cuda, off):
+    flat = torch.randint(-32768, 32768, (300 * 576 + 8,), device="cuda", dtype=torch.int16)
+    a = flat[off:off + 300 * 576].view(300, 576)
+    before, rest = a.clone(), flat.clone()
+    K.PoolMovePlan([37], [2], [260]).move(K.PoolSet.bf16([a]))
+    assert torch.equal(a[2:262], before[37:297]) and torch.equal(a[:2], before[:2]) and torch.equal(a[262:], before[262:])
+    assert torch.equal(flat[:off], rest[:off]) and torch.equal(flat[off + 300 * 576:], rest[off + 300 * 576:])
+
+
+def test_rows_too_wide_for_a_tile(K, torch_cuda):
+    a = torch.zeros(4, 4096, dtype=torch.int16, device="cuda")
+    with pytest.raises(K.KvlError, match="rows of 8192 bytes"):
+        K.PoolMovePlan([1], [0], [3]).move(K.PoolSet.bf16([a], 4032, 64))
