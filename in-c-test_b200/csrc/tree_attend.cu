@@ -485,6 +485,13 @@ __device__ __forceinline__ bool wait_full(Bars *B, uint32_t u, volatile int *abo
 // The latent ring runs in steps of two units, half a tile each.  An item is a
 // step of query boxes, which the issuer copies to tensor memory (tcgen05.cp),
 // then one step a tile.
+//
+// What bounds it.  One sequence of 131072 rows, 4 nodes: DRAM, 6.8 TB/s while the
+// tiles run, 39 us with the merge.  16 of 32768, 64 nodes: the tensor core, 1760
+// cycles of a tile's 2050, 1210 us (966 TFLOP/s) under the power cap.  64 of 512 to
+// 8192, 8 nodes: 119 us.  Q8 (4 of 32768, 32 nodes: 204 us): a tile takes 3300
+// cycles, for its scores wait until the softmax has read those before, and the
+// converters take issue slots and shared memory from both.
 template <bool Q8>
 __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __grid_constant__ TreeParams p) {
   extern __shared__ __align__(1024) uint8_t smem[];
