@@ -1002,23 +1002,29 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
     const int tid = (threadIdx.x - 32 * kConvertWarp) % kConvertThreads;
     const uint32_t odd = warp >= kConvertWarp + kConvertThreads / 32;
     const int box = lane >> 3, r = 4 * (tid >> 5) + (lane >> 1 & 3), half = lane & 1;
-    const long long last = p.rows - 1;
+    const uint32_t last = static_cast<uint32_t>(p.rows - 1);  // below 2^31
+    const int8_t *lat = p.lat8 + box * 64 + half * 32;
+    // the thread's first 16 bytes of row r in place 0; its others are an xor of bits 4-5 away
+    const uint32_t to = s_base + box * kBox + (r >> 3) * 1024 + (r & 7) * 128 + (((4 * half) ^ (r & 7)) << 4);
     const bool aligned = (reinterpret_cast<uintptr_t>(p.lat8) & 31) == 0;
     uint32_t j = 0, g = 0;
     bool ok = fit;
     for (int it = blockIdx.x; it >= 0 && ok; it = p.items[it].next) {
-      const long long row0 = p.items[it].row0;
+      const uint32_t row0 = static_cast<uint32_t>(p.items[it].row0);
       const int t0 = p.items[it].tile0, t1 = p.items[it].tile1;
       ++j;  // the query
       for (int t = t0; t < t1 && ok; ++t, ++j, ++g) {
         if ((g & 1) != odd) continue;
-        const long long first = row0 + static_cast<long long>(kTreeKeys) * t;
+        const uint32_t first = row0 + kTreeKeys * t;
         const float sc = tid < kTreeKeys ? __ldg(p.lscale + min(first + tid, last)) : 0.f;
         uint4 v[8];  // [unit][rows r and r + 32]
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          load_32(p.lat8 + min(first + r + 32 * (i & 1), last) * kLatent + (4 * (i >> 1) + box) * 64 + half * 32,
-                  aligned, v[2 * i], v[2 * i + 1]);
+        for (int i = 0; i < 2; ++i) {
+          const int8_t *src = lat + static_cast<size_t>(min(first + r + 32 * i, last)) * kLatent;
+          load_32(src, aligned, v[2 * i], v[2 * i + 1]);
+          load_32(src + 256, aligned, v[4 + 2 * i], v[5 + 2 * i]);
+        }
+        const uint32_t place = to + 2 * (j % (kUnits / 2)) * kUnit;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint32_t u = 2 * j + h;
@@ -1027,13 +1033,13 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
           if (h == 1 && tid < kTreeKeys) scales[g % kScaleRing][tid] = sc;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const int row = r + 32 * i;
-            uint8_t *dst = smem + (u % kUnits) * kUnit + box * kBox + (row >> 3) * 1024 + (row & 7) * 128;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               const uint4 x = v[4 * h + 2 * i + (c >> 1)];
               const uint2 lo = s8x4_to_bf16(c & 1 ? x.z : x.x), hi = s8x4_to_bf16(c & 1 ? x.w : x.y);
-              *reinterpret_cast<uint4 *>(dst + ((4 * half + c) ^ (row & 7)) * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"((place ^ (c << 4)) + h * kUnit + i * 4096),
+                           "r"(lo.x), "r"(lo.y), "r"(hi.x), "r"(hi.y)
+                           : "memory");
             }
           }
           fence_proxy_async_smem();
