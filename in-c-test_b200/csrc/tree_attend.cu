@@ -333,7 +333,12 @@ constexpr uint32_t kColS = 256, kColRope = kColS + 64, kColQ = kColS + 128;
 constexpr uint32_t kOddLanes = 16u << 16;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kU16 = kUnit / 16, kB16 = kBox / 16;  // in units of a matrix descriptor
-constexpr int kScaleRing = 3;
+// Row scales of the tiles between their conversion and their softmax.  A tile's
+// place in the ring of latents may have been the query's three steps before,
+// which is copied as soon as the scores of the last item are done: then the
+// third tile of an item is converted while the softmax has still to read the
+// scales of the last item's last one, so four sets, not three.
+constexpr int kScaleRing = 4;
 
 constexpr int kSoftThreads = 256;    // warps 4-11: softmax and epilogue
 constexpr int kConvertWarp = 12;       // Q8: warps 12-27 load and convert the latents,
@@ -341,11 +346,14 @@ constexpr int kConvertThreads = 256;   // 256 threads a CTA's even tiles, 256 th
 template <bool Q8>
 constexpr int threads() { return 128 + kSoftThreads + (Q8 ? 2 * kConvertThreads : 0); }
 
+constexpr uint32_t kSteps = 8;  // of the ring that have barriers of their own
+__device__ __forceinline__ uint32_t step_phase(uint32_t j) { return (j / kSteps) & 1; }
+
 struct Bars {
-  // of step j's unit h: [h][j % 4], phase j / 4.  full: its bytes are there; done:
+  // of step j's unit h: [h][j % 8], phase j / 8.  full: its bytes are there; done:
   // its half of the P.V (its copy to tensor memory) is, so its place is free
   // (unit 1: and the tile's rope)
-  uint64_t full[2][4], done[2][4];
+  uint64_t full[2][kSteps], done[2][kSteps];
   uint64_t qr_full, q_done;        // q_done: the item's last scores are done
   uint64_t s_full[2], s_empty[2];  // of tile g: [g % 2], phase g / 2
   uint64_t p_full, o_empty, drain[2];
@@ -459,14 +467,18 @@ struct Items {
   }
 };
 
-// Waits until unit u = 2 step + half is done (or full).  Steps share four
-// barriers, so nobody may ask for a step that is four or more behind the last
-// one loaded.
+// Waits until unit u = 2 step + half is done (or full).  Eight steps have
+// barriers of their own, so nobody may ask for a step that is eight or more
+// behind the last one done.  The softmax comes closest: before the first tile
+// of an item it asks for the step ahead of the query, while the scores may be
+// two tiles further and, where items have one tile, one query ahead of each of
+// them and of the next: seven steps.  (With four barriers, items of two tiles
+// ran past it.)
 __device__ __forceinline__ bool wait_done(Bars *B, uint32_t u, volatile int *abort, uint32_t *err) {
-  return mbar_wait(&B->done[u & 1][(u >> 1) & 3], (u >> 3) & 1, abort, err, ERR_TIMEOUT_EMPTY);
+  return mbar_wait(&B->done[u & 1][(u >> 1) % kSteps], step_phase(u >> 1), abort, err, ERR_TIMEOUT_EMPTY);
 }
 __device__ __forceinline__ bool wait_full(Bars *B, uint32_t u, volatile int *abort, uint32_t *err) {
-  return mbar_wait(&B->full[u & 1][(u >> 1) & 3], (u >> 3) & 1, abort, err, ERR_TIMEOUT_FULL);
+  return mbar_wait(&B->full[u & 1][(u >> 1) % kSteps], step_phase(u >> 1), abort, err, ERR_TIMEOUT_FULL);
 }
 
 // One CTA per SM, roles by warp:
@@ -522,7 +534,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
         if (!free_unit(h)) return false;
         // two pairs of boxes; a pair's rows alternate, 16 of the even box and 16
         // of the odd one, as their lanes do
-        uint64_t *full = &B->full[h][pj & 3];
+        uint64_t *full = &B->full[h][pj % kSteps];
         mbar_arrive_expect_tx(full, kUnit);
         for (int b = 0; b < 2; ++b)
           tma_load_5d(smem + ((2 * pj + h) % kUnits) * kUnit + b * 2 * kBox, &p.tm_q, full, 0, 0, 0, 2 * h + b, pim.node0);
@@ -535,13 +547,13 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
     const int32_t y = static_cast<int32_t>(pim.row0 + static_cast<long long>(kTreeKeys) * pt);
     for (int h = 0; h < 2 && !Q8; ++h) {
       if (!free_unit(h)) return false;
-      uint64_t *full = &B->full[h][pj & 3];
+      uint64_t *full = &B->full[h][pj % kSteps];
       mbar_arrive_expect_tx(full, kUnit + h * kBox);
       tma_load_3d(smem + ((2 * pj + h) % kUnits) * kUnit, &p.tm_lat, full, 0, y, 4 * h);
     }
     if (pg >= 2 && !mbar_wait(&B->s_full[pg & 1], ((pg >> 1) & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY)) return false;
-    if (Q8) mbar_arrive_expect_tx(&B->full[1][pj & 3], kBox);
-    tma_load_2d(smem + OFF_R + (pg & 1) * kBox, &p.tm_rope, &B->full[1][pj & 3], Q8 ? 0 : kLatent, y);
+    if (Q8) mbar_arrive_expect_tx(&B->full[1][pj % kSteps], kBox);
+    tma_load_2d(smem + OFF_R + (pg & 1) * kBox, &p.tm_rope, &B->full[1][pj % kSteps], Q8 ? 0 : kLatent, y);
     ++pt;
     ++pg;
     ++pj;
@@ -550,7 +562,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
 
   if (threadIdx.x == 0) {
     for (int h = 0; h < 2; ++h)
-      for (int i = 0; i < 4; ++i) {
+      for (uint32_t i = 0; i < kSteps; ++i) {
         mbar_init(&B->full[h][i], Q8 ? kConvertThreads / 32 + h : 1);  // + 1: the rope's
         mbar_init(&B->done[h][i], 1);
       }
@@ -624,8 +636,8 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
             for (int c = 0; c < 8; ++c)
               tmem_cp_128x128b(tmem + kColQ + 32 * b + 4 * c,
                                desc_of(k_lo + ((2 * j + (b >> 1)) % kUnits) * kU16 + (b & 1) * 2 * kB16 + c));
-          mma_commit(&B->done[0][j & 3]);
-          mma_commit(&B->done[1][j & 3]);
+          mma_commit(&B->done[0][j % kSteps]);
+          mma_commit(&B->done[1][j % kSteps]);
           ++j;
           for (int t = t0; t < t1; ++t, ++j, ++g) {
             // ---- S = Q . K^T
@@ -645,7 +657,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
 #pragma unroll
             for (int b = 0; b < 8; ++b) {
               const uint32_t s = (2 * j + (b >> 2)) % kUnits, odd = b & 1 ? kOddLanes : 0;
-              if (b == 3) hi_ok = mbar_test(&B->full[1][j & 3], (j >> 2) & 1);  // MMAs are queued meanwhile
+              if (b == 3) hi_ok = mbar_test(&B->full[1][j % kSteps], step_phase(j));  // MMAs are queued meanwhile
               if (b == 4) {
                 if (!hi_ok) ok = wait_full(B, 2 * j + 1, abort, p.err);
                 if (!ok) break;
@@ -697,7 +709,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
               for (int kk = 0; kk < 4; ++kk)
                 mma_f16_ws_ss(tmem + 128 * h, desc_of(pl + kk * 2), desc_of(vl + s * kU16 + kk * 128), id_pv,
                               t > t0 || kk > 0);
-              mma_commit(&B->done[h][j & 3]);
+              mma_commit(&B->done[h][j % kSteps]);
             }
           }
         }
@@ -835,7 +847,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
           need &= real;
           const bool vote = named_bar_or(1, kSoftThreads, need || bad);
           const uint32_t before = 2 * (t > tile0 ? j - 1 : j - 2) + 1;  // the P before is read until its P.V is done
-          const bool p_free = g == 0 || mbar_test(&B->done[1][(before >> 1) & 3], (before >> 3) & 1);
+          const bool p_free = g == 0 || mbar_test(&B->done[1][(before >> 1) % kSteps], step_phase(before >> 1));
           if (vote) {
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
@@ -1044,7 +1056,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&B->full[h][j & 3]);
+          if (lane == 0) mbar_arrive(&B->full[h][j % kSteps]);
         }
       }
     }

@@ -91,3 +91,18 @@ def test_negative_and_zero_row_scales(K, torch_cuda, q8):
         c.lscale[5::7] = 0
     c.run(c.plan(K), scale=-0.05)
     check(c, scale=-0.05)
+
+
+@pytest.mark.parametrize("q8", [False, True], ids=["bf16", "q8"])
+@pytest.mark.parametrize("ctas", [1, 2, 5])
+@pytest.mark.parametrize("tiles", [[2] * 12, [1] * 9, [3] * 6, [2, 1, 2, 2, 3, 1, 1, 2, 4, 2, 2, 5, 1, 2]])
+def test_short_items_follow_one_another(K, torch_cuda, q8, ctas, tiles):
+    """A CTA walks many sequences of few tiles: the roles of the kernel are as far apart as they get."""
+    lens = [64 * t - 20 for t in tiles]
+    c = Case(lens, [4] * len(lens), q8=q8, seed=len(lens) + ctas)
+    plan = c.plan(K, max_ctas=ctas)
+    for _ in range(5):
+        c.out.fill_(3)
+        c.run(plan)
+        assert plan.check() == 0
+    check(c)

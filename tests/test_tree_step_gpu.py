@@ -129,7 +129,8 @@ def path_to(parent, i):
 
 
 @pytest.mark.parametrize("q8", [False, True], ids=["bf16", "q8"])
-@pytest.mark.parametrize("lens,nodes", [([100], [1]), ([0, 37, 260], [3, 0, 8]), ([5, 64, 63, 0, 700], [4, 5, 1, 7, 33])])
+@pytest.mark.parametrize("lens,nodes", [([100], [1]), ([0, 37, 260], [3, 0, 8]), ([5, 64, 63, 0, 700], [4, 5, 1, 7, 33]),
+                                        ([90] * 40, [8] * 40), ([20] * 34, [64] * 34)])
 def test_step_decodes_every_path(K, torch_cuda, q8, lens, nodes):
     m = Model(K, 1, 21)
     row0, rows = layout(lens, nodes)
