@@ -548,7 +548,8 @@ KVL_EXPORT int kvl_mla_move_plan_create(KvlMlaMovePlan **plan, int runs, const i
     if (cudaGetDevice(&dev) != cudaSuccess || cudaMalloc(&p->d_mem, p->off_tiles + tile_bytes + 16) != cudaSuccess ||
         cudaMemset(p->d_mem, 0, p->off_tiles) != cudaSuccess ||
         (tile_bytes && cudaMemcpy(static_cast<uint8_t *>(p->d_mem) + p->off_tiles, p->tiles.data(), tile_bytes,
-                                  cudaMemcpyHostToDevice) != cudaSuccess)) {
+                                  cudaMemcpyHostToDevice) != cudaSuccess) ||
+        cudaStreamSynchronize(cudaStreamLegacy) != cudaSuccess) {  // the plan can be used on any stream afterwards
       cudaGetLastError();
       cudaFree(p->d_mem);
       delete p;
@@ -645,6 +646,7 @@ KVL_EXPORT int kvl_mla_move_check(const KvlMlaMovePlan *plan, void *stream) {
     return fail("move check: %s", cudaGetErrorString(cudaGetLastError()));
   if (err) {
     cudaMemset(plan->d_mem, 0, 4);
+    cudaStreamSynchronize(cudaStreamLegacy);
     return fail("pool move: device-side error 0x%x", err);
   }
   return 0;

@@ -61,8 +61,12 @@ static int upload(KvlMlaTreePlan &p) {
   if (cudaMalloc(&p.d_meta, at) != cudaSuccess) return -1;
   const size_t work = (size_t)h.slots * kTreeRows * (kLatent + 1) * sizeof(float);
   if (work && cudaMalloc(&p.d_work, work) != cudaSuccess) return -1;
-  // a blocking copy: the plan can be used on any stream afterwards
-  return cudaMemcpy(p.d_meta, stage.data(), at, cudaMemcpyHostToDevice) == cudaSuccess ? 0 : -1;
+  // The copy may return before its last bytes have arrived; the plan can be used
+  // on any stream afterwards, also on one that does not wait for this one.
+  return cudaMemcpy(p.d_meta, stage.data(), at, cudaMemcpyHostToDevice) == cudaSuccess &&
+                 cudaStreamSynchronize(cudaStreamLegacy) == cudaSuccess
+             ? 0
+             : -1;
 }
 
 static void release(KvlMlaTreePlan *p) {
@@ -237,6 +241,7 @@ KVL_EXPORT int kvl_mla_tree_check(const KvlMlaTreePlan *plan, void *stream) {
     return fail("tree check: %s", cudaGetErrorString(cudaGetLastError()));
   if (err) {
     cudaMemset(plan->d_meta, 0, 4);
+    cudaStreamSynchronize(cudaStreamLegacy);
     return fail("tree attend: device-side error 0x%x", err);
   }
   return 0;

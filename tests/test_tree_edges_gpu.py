@@ -106,3 +106,28 @@ def test_short_items_follow_one_another(K, torch_cuda, q8, ctas, tiles):
         c.run(plan)
         assert plan.check() == 0
     check(c)
+
+
+def test_plans_serve_other_streams_at_once(K, torch_cuda):
+    """Created and used at once on streams that do not wait for the default one, while that one is busy."""
+    c = Case([300, 5000], [9, 4], seed=41)
+    rows = torch.arange(20000 * 576, device="cuda", dtype=torch.int32).view(20000, 576).to(torch.int16)
+    want = rows[100:15100].clone()
+    busy = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for _ in range(5):
+            busy = busy @ busy * 1e-3
+        s = torch.cuda.Stream()
+        plan = c.plan(K)
+        c.run(plan, stream=s.cuda_stream)
+        move = K.PoolMovePlan([100], [50], [15000])
+        pool = rows.clone()
+        s.wait_stream(torch.cuda.current_stream())
+        move.move(K.PoolSet.bf16([pool]), stream=s.cuda_stream)
+        s.synchronize()
+        assert plan.check(s.cuda_stream) == 0 and move.check(s.cuda_stream) == 0
+        check(c)
+        assert torch.equal(pool[50:15050], want)
+        c.out.fill_(3)
+        torch.cuda.synchronize()
