@@ -499,9 +499,9 @@ __device__ __forceinline__ bool wait_full(Bars *B, uint32_t u, volatile int *abo
 // then one step a tile.
 //
 // What bounds it.  One sequence of 131072 rows, 4 nodes: DRAM, 6.8 TB/s while the
-// tiles run, 39 us with the merge.  16 of 32768, 64 nodes: the tensor core, 1760
-// cycles of a tile's 2050, 1210 us (966 TFLOP/s) under the power cap.  64 of 512 to
-// 8192, 8 nodes: 119 us.  Q8 (4 of 32768, 32 nodes: 204 us): a tile takes 3300
+// tiles run, 40 us with the merge.  16 of 32768, 64 nodes: the tensor core, 1760
+// cycles of a tile's 2050, 1227 us (952 TFLOP/s) under the power cap.  64 of 512 to
+// 8192, 8 nodes: 123 us.  Q8 (4 of 32768, 32 nodes: 201 us): a tile takes about 3200
 // cycles, for its scores wait until the softmax has read those before, and the
 // converters take issue slots and shared memory from both.
 template <bool Q8>
