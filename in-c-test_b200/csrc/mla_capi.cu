@@ -2053,7 +2053,8 @@ static int tree_step(const KvlMlaConfig *cfg, const KvlMlaDeviceWeights *w, cons
     return -1;
   }
   if (!plan->host.own_rows) {
-    set_err("tree step: two sequences of the plan have the same drafted row");
+    set_err("tree step: two sequences of the plan have the same drafted row, or one's drafted row is a cached row of "
+            "another");
     return -1;
   }
   int dev = -1;

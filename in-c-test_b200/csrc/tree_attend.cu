@@ -19,6 +19,29 @@ namespace kvl {
 // and read.
 static constexpr double kItemCost = 3.0, kMergeCost = 3.0, kSlotCost = 0.03;
 
+// Whether no drafted row is another sequence's drafted or cached row.  Cached
+// rows may be shared (a common prefix), and a sequence's own cached rows end
+// where its drafted ones begin.
+static bool drafted_rows_apart(const TreeHostPlan &hp) {
+  typedef std::pair<long long, long long> Range;  // [first, second)
+  std::vector<Range> drafted, cached;
+  for (int b = 0; b < hp.batch; ++b) {
+    const long long end = hp.row0[b] + hp.len[b];
+    if (hp.len[b]) cached.push_back({hp.row0[b], end});
+    if (hp.tree[b]) drafted.push_back({end, end + hp.tree[b]});
+  }
+  std::sort(drafted.begin(), drafted.end());
+  std::sort(cached.begin(), cached.end());
+  long long drafted_to = 0, cached_to = 0;  // ends of the ranges that begin before this one's end
+  size_t c = 0;
+  for (const Range &d : drafted) {
+    for (; c < cached.size() && cached[c].first < d.second; ++c) cached_to = std::max(cached_to, cached[c].second);
+    if (std::max(drafted_to, cached_to) > d.first) return false;
+    drafted_to = d.second;
+  }
+  return true;
+}
+
 int build_tree_plan(TreeHostPlan &hp, int batch, const int *cached_len, const int *nodes, const int64_t *row0,
                     int ctas) {
   if (batch <= 0 || ctas <= 0) return -1;
@@ -38,12 +61,7 @@ int build_tree_plan(TreeHostPlan &hp, int batch, const int *cached_len, const in
     hp.nodes += nodes[b];
   }
   if (hp.nodes == 0) return -1;
-  std::vector<std::pair<long long, int>> drafted;
-  for (int b = 0; b < batch; ++b)
-    if (nodes[b]) drafted.push_back({row0[b] + cached_len[b], nodes[b]});
-  std::sort(drafted.begin(), drafted.end());
-  for (size_t i = 1; i < drafted.size(); ++i)
-    hp.own_rows &= drafted[i - 1].first + drafted[i - 1].second <= drafted[i].first;
+  hp.own_rows = drafted_rows_apart(hp);
 
   struct Seq {
     int tiles, groups;

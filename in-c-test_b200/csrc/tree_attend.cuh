@@ -74,7 +74,7 @@ struct TreeHostPlan {
   std::vector<int> len, tree, seq_of_node, first_node;
   std::vector<long long> row0;
   long long rows_needed = 0;  // one past the last pool row that any sequence uses
-  bool own_rows = true;       // no two nodes have the same drafted row
+  bool own_rows = true;       // no drafted row is another sequence's drafted or cached row
 };
 
 int build_tree_plan(TreeHostPlan &hp, int batch, const int *cached_len, const int *nodes, const int64_t *row0,
