@@ -1,5 +1,5 @@
 // tree_attend.cuh -- attention of a tree of drafted tokens over the latent
-// cache: the work plan and the launchers (kernels in tree_attend.cu).
+// cache: the work plan (tree_plan.cu) and the launchers (kernels in tree_attend.cu).
 //
 // Sequence b has L_b cached rows at pool rows [row0_b, row0_b + L_b) and T_b
 // drafted rows right behind them.  Node i of its tree (head h) attends the
@@ -77,8 +77,10 @@ struct TreeHostPlan {
   bool own_rows = true;       // no drafted row is another sequence's drafted or cached row
 };
 
-int build_tree_plan(TreeHostPlan &hp, int batch, const int *cached_len, const int *nodes, const int64_t *row0,
-                    int ctas);
+// The plan in two steps (tree_plan.cu): the batch's sequences, -1 if one is out
+// of range, then its items for a grid of at most `ctas` >= 1.
+int set_tree_sequences(TreeHostPlan &hp, int batch, const int *cached_len, const int *nodes, const int64_t *row0);
+void deal_tree_tiles(TreeHostPlan &hp, int ctas);
 
 struct TreeGenericParams {
   const uint16_t *q;

@@ -70,8 +70,8 @@ static int upload(KvlMlaTreePlan &p) {
 }
 
 static void release(KvlMlaTreePlan *p) {
-  cudaFree(p->d_meta);
-  cudaFree(p->d_work);
+  if (p->d_meta) cudaFree(p->d_meta);
+  if (p->d_work) cudaFree(p->d_work);
   delete p;
 }
 
@@ -173,23 +173,25 @@ KVL_EXPORT int kvl_mla_tree_plan_create(KvlMlaTreePlan **plan, int batch, const 
   if (batch <= 0 || !cached_len || !nodes || !seq_row0 || num_heads <= 0 || num_heads > 65535 || kv_lora_rank <= 0 ||
       max_ctas < 0)
     return fail("tree plan: invalid arguments");
-  int dev = -1, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-    cudaGetLastError();
-    return fail("tree plan: no CUDA device");
-  }
   KvlMlaTreePlan *p = nullptr;
   try {
     p = new KvlMlaTreePlan();
-    p->device = dev;
-    p->nh = num_heads;
-    p->R = kv_lora_rank;
-    if (build_tree_plan(p->host, batch, cached_len, nodes, seq_row0, max_ctas > 0 ? max_ctas : sms) != 0) {
+    if (set_tree_sequences(p->host, batch, cached_len, nodes, seq_row0) != 0) {
       release(p);
       return fail("tree plan: cached lengths >= 0, 0 to %d nodes a sequence and one at least, rows >= 0 and below 2^31",
                   kTreeMaxNodes);
     }
+    int dev = -1, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+      cudaGetLastError();
+      release(p);
+      return fail("tree plan: no CUDA device");
+    }
+    p->device = dev;
+    p->nh = num_heads;
+    p->R = kv_lora_rank;
+    deal_tree_tiles(p->host, max_ctas > 0 ? max_ctas : sms);
     if (upload(*p) != 0) {
       cudaGetLastError();
       release(p);
