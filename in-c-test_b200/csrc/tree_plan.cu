@@ -15,6 +15,9 @@ namespace kvl {
 // and read.
 static constexpr double kItemCost = 3.0, kMergeCost = 3.0, kSlotCost = 0.03;
 
+// A list is kept per CTA, so a grid far beyond any GPU's SMs is cut to this.
+static constexpr int kMaxCtas = 1 << 16;
+
 // Whether no drafted row is another sequence's drafted or cached row.  Cached
 // rows may be shared (a common prefix), and a sequence's own cached rows end
 // where its drafted ones begin.
@@ -62,6 +65,7 @@ int set_tree_sequences(TreeHostPlan &hp, int batch, const int *cached_len, const
 
 void deal_tree_tiles(TreeHostPlan &hp, int ctas) {
   const int batch = hp.batch;
+  ctas = std::min(ctas, kMaxCtas);
   struct Seq {
     int tiles, groups;
   };
@@ -70,8 +74,9 @@ void deal_tree_tiles(TreeHostPlan &hp, int ctas) {
   int longest = 1, groups = 0;
   bool uniform = true;  // all sequences with drafted rows have as many groups
   for (int b = 0; b < batch; ++b) {
-    const int keys = hp.len[b] + hp.tree[b];
-    seqs[b] = {hp.tree[b] ? (keys + kTreeKeys - 1) / kTreeKeys : 0, (hp.tree[b] + kTreeGroup - 1) / kTreeGroup};
+    const long long keys = (long long)hp.len[b] + hp.tree[b];  // up to 2^31 - 1, and kTreeKeys more
+    seqs[b] = {hp.tree[b] ? (int)((keys + kTreeKeys - 1) / kTreeKeys) : 0,
+               (hp.tree[b] + kTreeGroup - 1) / kTreeGroup};
     total += (long long)seqs[b].tiles * seqs[b].groups;
     longest = std::max(longest, seqs[b].tiles);
     if (seqs[b].groups) {

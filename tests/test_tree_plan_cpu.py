@@ -142,6 +142,14 @@ def test_sequences_around_the_tiles(dump):
         check_plan(*b, p)
 
 
+def test_longest_sequence_and_largest_grid(dump):
+    """Key counts up to the last row below 2^31, and a grid that no list of CTAs could be kept for."""
+    batches = [([n], [t], [0], c) for n, t in ((2 ** 31 - 65, 64), (2 ** 31 - 2, 1), (2 ** 31 - 40, 5)) for c in (1, 148)]
+    batches += [([700, 20], [5, 1], [0, 800], 2 ** 31 - 1), ([0], [1], [0], 2 ** 31 - 1)]
+    for b, p in zip(batches, dump(batches)):
+        check_plan(*b, p)
+
+
 def test_whose_rows_a_sequence_may_append_to(dump):
     """own: no drafted row is another sequence's drafted or cached row, against all pairs."""
     r = np.random.RandomState(8)
