@@ -1766,8 +1766,9 @@ static bool step_gemm_ok(const KvlMlaConfig &c, const KvlMlaDeviceWeights &w, co
   const uintptr_t a = reinterpret_cast<uintptr_t>(w.q_proj) | reinterpret_cast<uintptr_t>(w.kv_a_proj) |
                       reinterpret_cast<uintptr_t>(w.kv_b_proj) | reinterpret_cast<uintptr_t>(w.o_proj) |
                       reinterpret_cast<uintptr_t>(d_out) | reinterpret_cast<uintptr_t>(ws);
-  // 16-byte tensor-map bases and row strides, 16-byte vector stores
-  return (a & 15) == 0 && c.hidden_size % 8 == 0 && c.qk_nope_dim % 8 == 0 &&
+  // 16-byte tensor-map bases and row strides, 16-byte vector stores; the products
+  // per head (absorb, V up-projection) are one batched launch of two heads at least
+  return (a & 15) == 0 && c.num_heads > 1 && c.hidden_size % 8 == 0 && c.qk_nope_dim % 8 == 0 &&
          c.qk_rope_dim % 8 == 0 && c.kv_lora_rank % 8 == 0 && c.v_head_dim % 8 == 0;
 }
 
@@ -2068,7 +2069,8 @@ static int tree_step(const KvlMlaConfig *cfg, const KvlMlaDeviceWeights *w, cons
       ((reinterpret_cast<uintptr_t>(d_x) | reinterpret_cast<uintptr_t>(d_pos) |
         reinterpret_cast<uintptr_t>(pool.lscale)) & 3) ||
       (reinterpret_cast<uintptr_t>(d_mask) & 7)) {
-    set_err("tree step: weights, output, workspace and pool must be 16-byte aligned and every width a multiple of 8");
+    set_err("tree step: weights, output, workspace and pool must be 16-byte aligned, every width a multiple of 8 and "
+            "the heads two at least");
     return -1;
   }
   const int nodes = plan->host.nodes;

@@ -264,8 +264,8 @@ int kvl_mla_tree_attend_q8(const KvlMlaTreePlan *plan, uint16_t *d_out, float *d
  * node's depth), attend under d_mask, V up-projection and o_proj.  d_x/d_out
  * [nodes][H] fp32, d_pos [nodes].  The projections run as tensor-core GEMMs on
  * bf16-rounded activations for any number of nodes: weights, d_out, workspace
- * and pool 16-byte aligned, every width a multiple of 8, else -1 before
- * anything is launched.  Sequences may share cached rows (a common prefix); a
+ * and pool 16-byte aligned, every width a multiple of 8, two heads at least,
+ * else -1 before anything is launched.  Sequences may share cached rows (a common prefix); a
  * plan where a drafted row of one is a drafted or cached row of another is
  * refused, for its append would overwrite the other's.  Workspace of
  * kvl_mla_decode_step_workspace_bytes(cfg, nodes).  Device-side errors are
