@@ -170,6 +170,7 @@ struct Bars {
   uint32_t tmem_base;
   int abort;
   uint32_t nonfinite[8];
+  uint32_t cleared[2][kTreeGroup][2];  // [tile % 2][node][key half]: rows cleared that the node sees
   float red[2][2][kTreeRows];  // row maxima or sums of the two key halves, alternate exchanges
   float alpha[kTreeRows];
 };
@@ -570,6 +571,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
         const bool real = sub < p.items[it].nn;  // or the rows hold whatever was there
         float m[2] = {-INFINITY, -INFINITY};
         float2 l[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        uint32_t cleared = 0;  // bit z: some rows of the item's masked tile with t % 2 = z (it has two at most)
         for (int t = tile0; t < tile1; ++t, ++g, ++j) {
           bad |= !mbar_wait(&B->s_full[g & 1], (g >> 1) & 1, abort, p.err, ERR_TIMEOUT_MMA);
           tc_fence_after();
@@ -611,7 +613,8 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
               // A hidden row gets p = 0, but 0 times an infinity or a NaN of the
               // row itself is NaN in the P.V product.  Such a row gives a score
               // that is not finite with every query (a query that is not finite
-              // does so with every row, but only its own): clear those rows.
+              // does so with every row, but only its own): clear those rows.  A
+              // node that does see one gets its part at the item's end.
               uint32_t nf[2] = {0, 0};
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
@@ -632,6 +635,9 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
                 uint8_t *v0 = smem + ((2 * j + (box >> 2)) % kUnits) * kUnit + (box & 3) * kBox + (tid & 7) * 16;
                 for (int k = tid >> 6; k < kTreeKeys; k += 4)
                   if (rows[k >> 5] >> (k & 31) & 1) *reinterpret_cast<uint4 *>(v0 + k * 128) = make_uint4(0u, 0u, 0u, 0u);
+                if (lane == 0)
+                  B->cleared[t & 1][sub][kh] = static_cast<uint32_t>(vis >> (32 * kh)) & (kh ? rows[1] : rows[0]);
+                cleared |= 1u << (t & 1);
               }
             }
           }
@@ -781,6 +787,25 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
           tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[i] *= inv;
+          // A cleared row that the node sees scored -inf, with weight 0 (or its
+          // weight was NaN, and so is all of o): 0 times its elements is NaN where
+          // they are not finite, whatever other nodes of the group see.
+          if (!Q8 && cleared)
+            for (int z = 0; z < 2; ++z) {
+              if (!(cleared >> z & 1)) continue;
+              const int last = im.tile1 - 1;
+              const uint16_t *v0 = p.kv + (im.row0 + kTreeKeys * (last - ((last ^ z) & 1))) * kRow + odim + c;
+              for (int half = 0; half < 2; ++half)
+                for (uint32_t w = B->cleared[z][orow >> 4][half]; w; w &= w - 1) {
+                  const uint16_t *v = v0 + (32 * half + __ffs(w) - 1) * kRow;
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) o[i] = fmaf(0.f, __bfloat162float(__ushort_as_bfloat16(v[i])), o[i]);
+                }
+            }
+          if (lo == 0.f && im.slot < 0) {  // all scores -inf, and O may hold 0 * inf
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = 0.f;
+          }
           if (staged) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -994,6 +1019,7 @@ __global__ void __launch_bounds__(LANES * Z) tree_merge_kernel(uint16_t *out, fl
   if (!real) return;
   const size_t orow = static_cast<size_t>(e.node0) * kHeads + row;
   if (lse && quad == 0 && half == 0) lse[orow] = sum == 0.f ? -INFINITY : m + logf(sum);
+  if (sum == 0.f) acc = make_float4(0.f, 0.f, 0.f, 0.f);  // also where a part holds 0 * inf
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   const int c = 4 * quad;  // the attend lane's column
   *reinterpret_cast<uint2 *>(out + orow * kLatent + (c >> 7) * 256 + half * 128 + (c & 127)) =

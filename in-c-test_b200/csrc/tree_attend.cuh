@@ -52,6 +52,7 @@ struct TreeParams {
   CUtensorMap tm_q;     // the query's latents: [node][pair of boxes][odd][16 heads][64], a load: 4 x 1 x 2 x 16 x 64
   CUtensorMap tm_qr;    // its rope: 64 rows (4 nodes) x 64
   CUtensorMap tm_out;   // out [nodes * 16][512]: 16 rows x 64 dims
+  const uint16_t *kv;   // bf16 pool, or
   const int8_t *lat8;   // Q8 pool
   const float *lscale;
   const uint64_t *mask; // [nodes]

@@ -103,6 +103,7 @@ static int attend(const KvlMlaTreePlan *plan, uint16_t *out, float *lse, const u
     std::memset(&p, 0, sizeof p);
     const bool q8 = !kv;
     if (!tree_maps(p, q, kv, rope16, out, plan->host.nodes, rows)) return fail("tree attend: tensor map");
+    p.kv = kv;
     p.lat8 = lat8;
     p.lscale = lscale;
     p.mask = mask;

@@ -241,10 +241,11 @@ int kvl_mla_tree_mask(uint64_t *mask, const int *parent, int nodes);
 
 /* d_q [nodes][num_heads][kv_lora_rank + rope_dim] bf16 absorbed queries, d_mask
  * [nodes], d_out [nodes][num_heads][kv_lora_rank] bf16, d_lse [nodes]
- * [num_heads] (natural log; may be NULL).  A node that attends no row gets 0
- * and -inf.  What lies in rows that a node does not attend, infinities and NaN
- * included, does not reach its result; rows behind the drafted ones are not
- * used.  Scores, softmax sums and the accumulation are fp32; the softmax
+ * [num_heads] (natural log; may be NULL).  A node that attends no row, or none
+ * with a score above -inf, gets 0 and -inf.  What lies in rows that a node does
+ * not attend, infinities and NaN included, does not reach its result; rows that
+ * it does attend count as in the formula (0 times an infinity is NaN), whatever
+ * other nodes attend.  Rows behind the drafted ones are not used.  Scores, softmax sums and the accumulation are fp32; the softmax
  * weights enter the P.V product as bf16.  The production shape (16, 512, 64)
  * runs on the tensor cores and wants d_q, d_out and the pool's arrays 16-byte
  * aligned; other shapes run a CUDA-core kernel.  The outputs overlap no input.  A device-side error is
