@@ -275,7 +275,15 @@ class CompressedState:
 
 def t_ptr(t) -> int:
     """Device pointer of a torch tensor (0 for None)."""
-    return 0 if t is None else int(t.data_ptr())
+    return 0 if t is None else t.data_ptr()
+
+
+def dense(what: str, *tensors) -> None:
+    """Raises unless every (name, tensor, bytes) is a contiguous tensor on a GPU of that many bytes at least (the library
+    takes bare pointers); a tensor that is None is left to the library."""
+    for name, t, n in tensors:
+        if t is not None and not (t.is_cuda and t.is_contiguous() and t.nbytes >= n):
+            raise KvlError(f"{what}: {name} must be contiguous, on a GPU, and have {n} bytes at least")
 
 
 class PeerGroup:
@@ -380,6 +388,8 @@ class TreePlan:
             raise KvlError("tree plan: cached_len, nodes and seq_row0 have one entry per sequence")
         self.batch, self.nodes = int(cl.shape[0]), int(nn.sum())
         self.num_heads, self.kv_lora_rank = num_heads, kv_lora_rank
+        self.query_rows = self.nodes * num_heads  # of all nodes
+        self.out_bytes, self.lse_bytes, self.mask_bytes = 2 * self.query_rows * kv_lora_rank, 4 * self.query_rows, 8 * self.nodes
         check(self.lib.kvl_mla_tree_plan_create(C.byref(self.h), self.batch, ptr(cl, i32p), ptr(nn, i32p),
                                                 ptr(r0, i64p), num_heads, kv_lora_rank, max_ctas), "tree plan create")
 
@@ -389,23 +399,40 @@ class TreePlan:
         return {"ctas": a.value, "partials": b.value, "items": c.value}
 
     def attend_bf16(self, out, lse, q, mask, kv, rows, rope_dim=64, scale=1.0 / np.sqrt(192.0), stream=0):
+        width = 2 * (self.kv_lora_rank + rope_dim)
+        dense("tree attend", ("out", out, self.out_bytes), ("lse", lse, self.lse_bytes), ("q", q, self.query_rows * width),
+              ("mask", mask, self.mask_bytes), ("kv", kv, rows * width))
         check(self.lib.kvl_mla_tree_attend_bf16(self.h, t_ptr(out), t_ptr(lse), t_ptr(q), t_ptr(mask), t_ptr(kv),
                                                 rows, self.num_heads, self.kv_lora_rank, rope_dim, float(scale),
                                                 stream), "tree attend")
 
     def attend_q8(self, out, lse, q, mask, lat8, lscale, rope16, rows, rope_dim=64, scale=1.0 / np.sqrt(192.0),
                   stream=0):
+        dense("tree attend", ("out", out, self.out_bytes), ("lse", lse, self.lse_bytes),
+              ("q", q, self.query_rows * 2 * (self.kv_lora_rank + rope_dim)), ("mask", mask, self.mask_bytes),
+              ("lat8", lat8, rows * self.kv_lora_rank), ("lscale", lscale, 4 * rows),
+              ("rope16", rope16, 2 * rows * rope_dim))
         check(self.lib.kvl_mla_tree_attend_q8(self.h, t_ptr(out), t_ptr(lse), t_ptr(q), t_ptr(mask), t_ptr(lat8),
                                               t_ptr(lscale), t_ptr(rope16), rows, self.num_heads, self.kv_lora_rank,
                                               rope_dim, float(scale), stream), "tree attend")
 
+    def _step_sizes(self, cfg, out, x, mask, pos, workspace):
+        n = 4 * self.nodes * cfg.hidden_size
+        size = self.lib.kvl_mla_decode_step_workspace_bytes(C.byref(cfg), self.nodes)
+        dense("tree step", ("out", out, n), ("x", x, n), ("mask", mask, 0), ("pos", pos, 0), ("workspace", workspace, size))
+
     def step_bf16(self, cfg, weights, out, x, mask, pos, kv, rows, workspace, stream=0):
-        """kvl_mla_tree_step_bf16: cfg a KvlMlaConfig, weights a KvlMlaDeviceWeights, workspace of
-        kvl_mla_decode_step_workspace_bytes(cfg, nodes) bytes."""
+        """kvl_mla_tree_step_bf16: cfg a KvlMlaConfig, weights a KvlMlaDeviceWeights, mask and pos one element a node,
+        workspace of kvl_mla_decode_step_workspace_bytes(cfg, nodes) bytes."""
+        self._step_sizes(cfg, out, x, mask, pos, workspace)
+        dense("tree step", ("kv", kv, 2 * rows * (cfg.kv_lora_rank + cfg.qk_rope_dim)))
         check(self.lib.kvl_mla_tree_step_bf16(C.byref(cfg), C.byref(weights), self.h, t_ptr(out), t_ptr(x), t_ptr(mask),
                                               t_ptr(pos), t_ptr(kv), rows, t_ptr(workspace), stream), "tree step")
 
     def step_q8(self, cfg, weights, out, x, mask, pos, lat8, lscale, rope16, rows, workspace, stream=0):
+        self._step_sizes(cfg, out, x, mask, pos, workspace)
+        dense("tree step", ("lat8", lat8, rows * cfg.kv_lora_rank), ("lscale", lscale, 4 * rows),
+              ("rope16", rope16, 2 * rows * cfg.qk_rope_dim))
         check(self.lib.kvl_mla_tree_step_q8(C.byref(cfg), C.byref(weights), self.h, t_ptr(out), t_ptr(x), t_ptr(mask),
                                             t_ptr(pos), t_ptr(lat8), t_ptr(lscale), t_ptr(rope16), rows,
                                             t_ptr(workspace), stream), "tree step")
@@ -433,10 +460,14 @@ class PoolSet:
         self.n, self.rows = len(first), int(first[0].shape[0]) if first else 0
         for a in self.tensors:
             for t in a:
-                if len(a) != self.n or int(t.shape[0]) != self.rows or not t.is_contiguous():
-                    raise KvlError("pool set: contiguous arrays with the same number of pools and rows")
+                if len(a) != self.n or int(t.shape[0]) != self.rows or not t.is_contiguous() or not t.is_cuda:
+                    raise KvlError("pool set: contiguous arrays on a GPU with the same number of pools and rows")
         self.rank, self.rope = widths
         self.ptrs = [(C.c_void_p * self.n)(*[t.data_ptr() for t in a]) for a in self.tensors]
+        # the arguments that say where the pools lie, converted once
+        self.head = (*[C.cast(p, C.c_void_p) for p in self.ptrs], C.c_int(self.n), C.c_int64(self.rows),
+                     C.c_int(self.rank), C.c_int(self.rope))
+        self.accept = self.lib.kvl_mla_tree_accept_bf16 if len(self.ptrs) == 1 else self.lib.kvl_mla_tree_accept_q8
 
     @classmethod
     def bf16(cls, kv, kv_lora_rank=512, rope_dim=64, lib=None):
@@ -460,9 +491,13 @@ class PoolSet:
     def tree_accept(self, base, path, count, kept=None, stream=0):
         """kvl_mla_tree_accept_*: base int64 [batch], path int32 [batch][max_path], count int32 [batch], kept int32
         [batch] or None, on the device."""
-        fn = self.lib.kvl_mla_tree_accept_bf16 if len(self.ptrs) == 1 else self.lib.kvl_mla_tree_accept_q8
-        check(fn(*self.ptrs, self.n, self.rows, self.rank, self.rope, int(base.shape[0]), t_ptr(base), t_ptr(path),
-                 t_ptr(count), int(path.shape[1]), t_ptr(kept), stream), "tree accept")
+        batch, width = base.shape[0], path.shape[1]
+        dense("tree accept", ("base", base, 8 * batch), ("path", path, 4 * batch * width), ("count", count, 4 * batch),
+              ("kept", kept, 4 * batch))
+        if path.itemsize != 4 or count is not None and count.itemsize != 4:
+            raise KvlError("tree accept: path and count are int32")
+        check(self.accept(*self.head, batch, base.data_ptr(), path.data_ptr(), t_ptr(count), width, t_ptr(kept), stream),
+              "tree accept")
 
 
 class PoolMovePlan:
@@ -484,7 +519,7 @@ class PoolMovePlan:
 
     def move(self, pools: PoolSet, stream=0):
         fn = self.lib.kvl_mla_pool_move_bf16 if len(pools.ptrs) == 1 else self.lib.kvl_mla_pool_move_q8
-        check(fn(self.h, *pools.ptrs, pools.n, pools.rows, pools.rank, pools.rope, stream), "pool move")
+        check(fn(self.h, *pools.head, stream), "pool move")
 
     def check(self, stream=0):
         return self.lib.kvl_mla_move_check(self.h, stream)
