@@ -10,9 +10,10 @@
 
 namespace kvl {
 
-// In tiles (about 1.2 us): what an item costs beside its tiles (query, first
-// tile, epilogue), what the merge launch costs, and a partial's 131 KB written
-// and read.
+// In tiles (bf16 about 1.2 us, Q8 about 1.7): what an item costs beside its tiles
+// (query, first tile, epilogue), what the merge launch costs, and a partial's 131
+// KB written and read.  Estimates from the traces of bf16 runs, used for Q8 too: a
+// plan does not know the pool that it will read.
 static constexpr double kItemCost = 3.0, kMergeCost = 3.0, kSlotCost = 0.03;
 
 // A list is kept per CTA, so a grid far beyond any GPU's SMs is cut to this.
