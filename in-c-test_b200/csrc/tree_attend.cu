@@ -128,7 +128,7 @@ constexpr uint32_t kUnit = 4 * kBox;        // half a tile's latents: 64 rows x 
 // scores and P.V of a tile in turn, a tile took 3420 cycles, of which the tensor
 // core worked about 1750).
 constexpr int kUnits = 6;
-constexpr uint32_t OFF_R = kUnits * kUnit;  // ropes of two tiles, until their scores are done
+constexpr uint32_t OFF_R = kUnits * kUnit;  // ropes of two tiles, until their scores are done; Q8: then the weights' second part
 constexpr uint32_t OFF_P = OFF_R + 2 * kBox;
 constexpr uint32_t OFF_QR = OFF_P + kBox;   // the query's rope box
 constexpr uint32_t OFF_BAR = OFF_QR + kBox;
@@ -165,11 +165,12 @@ constexpr uint32_t kSteps = 8;  // of the ring that have barriers of their own
 __device__ __forceinline__ uint32_t step_phase(uint32_t j) { return (j / kSteps) & 1; }
 
 struct Bars {
-  // of step j's unit h: [h][j % 8], phase j / 8.  full: its bytes are there (unit
-  // 1: and the tile's rope); done: its half of the P.V (its copy to tensor memory)
-  // is, so its place is free.  The rope's place is free once the scores are
-  // (s_full)
+  // of step j's unit h: [h][j % 8], phase j / 8.  full: its bytes are there (bf16,
+  // unit 1: and the tile's rope); done: its half of the P.V (its copy to tensor
+  // memory) is, so its place is free (Q8, unit 1: and the rope's place, where the
+  // weights' second part lay; bf16: that is free once the scores are)
   uint64_t full[2][kSteps], done[2][kSteps];
+  uint64_t r_full[2];              // Q8: the rope of tile g is there: [g % 2], phase g / 2
   uint64_t qr_full, q_done;        // q_done: the item's last scores are done
   uint64_t s_full[2], s_empty[2];  // of tile g: [g % 2], phase g / 2
   uint64_t p_full, o_empty, drain[2];
@@ -322,7 +323,7 @@ __device__ __forceinline__ bool wait_full(Bars *B, uint32_t u, volatile int *abo
 // What bounds it.  One sequence of 131072 rows, 4 nodes: DRAM, 6.8 TB/s while the
 // tiles run, 40 us with the merge.  16 of 32768, 64 nodes: the tensor core, 1760
 // cycles of a tile's 2050, 1227 us (952 TFLOP/s) under the power cap.  64 of 512 to
-// 8192, 8 nodes: 123 us.  Q8 (4 of 32768, 32 nodes: 201 us): a tile takes about 3200
+// 8192, 8 nodes: 124 us.  Q8 (4 of 32768, 32 nodes: 234 us): a tile takes about 3700
 // cycles, for its scores wait until the softmax has read those before, and the
 // converters take issue slots and shared memory from both.
 template <bool Q8>
@@ -341,6 +342,7 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
   pim.tile1 = 0;
   int pt = 0;
   uint32_t pg = 0, pj = 0;  // tiles and steps issued
+  uint32_t step1 = 0, step2 = 0;  // steps of the last tile issued and of the one before
   auto produce = [&]() -> bool {
     // the places of step pj: their last steps must be done
     auto free_unit = [&](int h) -> bool {
@@ -359,8 +361,8 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
         mbar_arrive_expect_tx(full, kUnit);
         for (int b = 0; b < 2; ++b)
           tma_load_5d(smem + ((2 * pj + h) % kUnits) * kUnit + b * 2 * kBox, &p.tm_q, full, 0, 0, 0, 2 * h + b, pim.node0);
-        if (Q8)  // the barrier counts the converter warps, and the rope's arrival
-          for (int i = 1; i < kConvertThreads / 32 + h; ++i) mbar_arrive(full);
+        if (Q8)  // the barrier counts the converter warps
+          for (int i = 1; i < kConvertThreads / 32; ++i) mbar_arrive(full);
       }
       ++pj;
       return true;
@@ -372,9 +374,24 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
       mbar_arrive_expect_tx(full, kUnit + h * kBox);
       tma_load_3d(smem + ((2 * pj + h) % kUnits) * kUnit, &p.tm_lat, full, 0, y, 4 * h);
     }
-    if (pg >= 2 && !mbar_wait(&B->s_full[pg & 1], ((pg >> 1) & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY)) return false;
-    if (Q8) mbar_arrive_expect_tx(&B->full[1][pj % kSteps], kBox);
-    tma_load_2d(smem + OFF_R + (pg & 1) * kBox, &p.tm_rope, &B->full[1][pj % kSteps], Q8 ? 0 : kLatent, y);
+    if constexpr (Q8) {
+      // The rope goes where the second part of the weights of tile pg - 2 lies until
+      // its P.V is done, about when the scores of tile pg begin, which need it last:
+      // its way from DRAM is taken one tile earlier.
+      if (pt + 1 < pim.tile1)
+        tma_prefetch_l2_2d(&p.tm_rope, 0, y + kTreeKeys);
+      else if (pim.next >= 0)
+        tma_prefetch_l2_2d(&p.tm_rope, 0,
+                           static_cast<int32_t>(p.items[pim.next].row0 + kTreeKeys * p.items[pim.next].tile0));
+      if (pg >= 2 && !wait_done(B, 2 * step2 + 1, abort, p.err)) return false;
+      step2 = step1;
+      step1 = pj;
+      mbar_arrive_expect_tx(&B->r_full[pg & 1], kBox);
+      tma_load_2d(smem + OFF_R + (pg & 1) * kBox, &p.tm_rope, &B->r_full[pg & 1], 0, y);
+    } else {
+      if (pg >= 2 && !mbar_wait(&B->s_full[pg & 1], ((pg >> 1) & 1) ^ 1, abort, p.err, ERR_TIMEOUT_EMPTY)) return false;
+      tma_load_2d(smem + OFF_R + (pg & 1) * kBox, &p.tm_rope, &B->full[1][pj % kSteps], kLatent, y);
+    }
     ++pt;
     ++pg;
     ++pj;
@@ -384,12 +401,13 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
   if (threadIdx.x == 0) {
     for (int h = 0; h < 2; ++h)
       for (uint32_t i = 0; i < kSteps; ++i) {
-        mbar_init(&B->full[h][i], Q8 ? kConvertThreads / 32 + h : 1);  // + 1: the rope's
+        mbar_init(&B->full[h][i], Q8 ? kConvertThreads / 32 : 1);
         mbar_init(&B->done[h][i], 1);
       }
     mbar_init(&B->qr_full, 1);
     mbar_init(&B->q_done, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&B->r_full[i], 1);
       mbar_init(&B->s_full[i], 1);
       mbar_init(&B->s_empty[i], kSoftThreads / 32);
     }
@@ -489,6 +507,10 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
                 mma_f16_ts(s_lat + odd, tq + 32 * (b >> 1) + 8 * kk + odd,
                            desc_of(kl + s * kU16 + (b & 3) * kB16 + kk * 2), id_qk, b > 1 || kk > 0);
             }
+            if (Q8 && ok) {
+              ok = mbar_wait(&B->r_full[g & 1], (g >> 1) & 1, abort, p.err, ERR_TIMEOUT_FULL);
+              tc_fence_after();
+            }
             if (!ok) break;
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
@@ -521,15 +543,22 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
                    mbar_wait(&B->p_full, g & 1, abort, p.err, ERR_TIMEOUT_FULL);
             if (!ok) break;
             tc_fence_after();
-            uint32_t pl = p_lo, vl = v_lo;
-            asm volatile("" : "+r"(pl), "+r"(vl));
+            uint32_t pl = p_lo, vl = v_lo, p2 = p_lo + (OFF_R + (g & 1) * kBox - OFF_P) / 16;
+            asm volatile("" : "+r"(pl), "+r"(vl), "+r"(p2));
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const uint32_t s = (2 * j + h) % kUnits;
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                mma_f16_ws_ss(tmem + 128 * h, desc_of(pl + kk * 2), desc_of(vl + s * kU16 + kk * 128), id_pv,
-                              t > t0 || kk > 0);
+              for (int kk = 0; kk < 4; ++kk) {
+                const uint64_t v = desc_of(vl + s * kU16 + kk * 128);
+                const uint32_t acc = t > t0 || kk > 0;
+                if (!Q8)
+                  mma_f16_ws_ss(tmem + 128 * h, desc_of(pl + kk * 2), v, id_pv, acc);
+                else if (kk & 1)
+                  mma_f16_ws_ss_two<1>(tmem + 128 * h, desc_of(pl + kk * 2), desc_of(p2 + kk * 2), v, id_pv, acc);
+                else
+                  mma_f16_ws_ss_two<0>(tmem + 128 * h, desc_of(pl + kk * 2), desc_of(p2 + kk * 2), v, id_pv, acc);
+              }
               mma_commit(&B->done[h][j % kSteps]);
             }
           }
@@ -738,16 +767,30 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
             if (masked) clear_hidden();  // a hidden row's scale may be anything
           }
           if (!p_free) bad |= !wait_done(B, before, abort, p.err);
-          // The weights enter P.V as bf16, the type of the rows they meet (Q8: after
-          // the row scale, so that the int8 rows need none); their sums l stay fp32.
-          // Each is off by 2^-8 at most, 1.6e-3 in the root mean square, as is the
-          // bf16 output: 0.0017 to 0.0023 in all against 64 bits, 0.0017 with the
-          // output's rounding alone.  Two bf16 parts would double the P.V products.
-          const uint32_t pd = s_base + OFF_P + 2 * sub * 1024 + (lane & 7) * 128 + (((4 * kh + (lane >> 3)) ^ (lane & 7)) * 16);
+          // The weights enter P.V as bf16, the type of the rows they meet; their sums l
+          // stay fp32.  A weight is off by 2^-8 at most, 1.6e-3 in the root mean square,
+          // like a bf16 output.  bf16 rows: 0.0017 to 0.0019 in all against 64 bits,
+          // 0.0017 with the output's rounding alone (the reference weight is 1, exactly).
+          // Q8 weights carry the row scale, so that the int8 rows need none, and are all
+          // off: 0.0018 to 0.0025, in short sequences up to twice the output's rounding.
+          // What the first part leaves goes in as a second one, 16 bits in all: 0.0017;
+          // 4 x 32768 rows, 32 nodes 202 -> 234 us, 64 x 512-8192, 4 nodes 78 -> 88 us
+          // (the second products without the collector: 255 and 92).
+          const uint32_t at = 2 * sub * 1024 + (lane & 7) * 128 + (((4 * kh + (lane >> 3)) ^ (lane & 7)) * 16);
 #pragma unroll
-          for (int y = 0; y < 2; ++y)
-            stmatrix_x4(pd + y * 1024, pack_bf16(s[y].x, s[y].y), pack_bf16(s[2 + y].x, s[2 + y].y),
-                        pack_bf16(s[4 + y].x, s[4 + y].y), pack_bf16(s[6 + y].x, s[6 + y].y));
+          for (int y = 0; y < 2; ++y) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = pack_bf16(s[2 * i + y].x, s[2 * i + y].y);
+            stmatrix_x4(s_base + OFF_P + at + y * 1024, w[0], w[1], w[2], w[3]);
+            if constexpr (Q8) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                w[i] = pack_bf16(s[2 * i + y].x - __uint_as_float(w[i] << 16),
+                                 s[2 * i + y].y - __uint_as_float(w[i] & 0xffff0000u));
+              stmatrix_x4(s_base + OFF_R + (g & 1) * kBox + at + y * 1024, w[0], w[1], w[2], w[3]);
+            }
+          }
           fence_proxy_async_smem();
           tc_fence_before();
           __syncwarp();

@@ -245,10 +245,12 @@ int kvl_mla_tree_mask(uint64_t *mask, const int *parent, int nodes);
  * with a score above -inf, gets 0 and -inf.  What lies in rows that a node does
  * not attend, infinities and NaN included, does not reach its result; rows that
  * it does attend count as in the formula (0 times an infinity is NaN), whatever
- * other nodes attend.  Rows behind the drafted ones are not used.  Scores, softmax sums and the accumulation are fp32; the softmax
- * weights enter the P.V product as bf16.  The production shape (16, 512, 64)
- * runs on the tensor cores and wants d_q, d_out and the pool's arrays 16-byte
- * aligned; other shapes run a CUDA-core kernel.  The outputs overlap no input.  A device-side error is
+ * other nodes attend.  Rows behind the drafted ones are not used.
+ * Scores, softmax sums and the accumulation are fp32; the softmax weights enter
+ * the P.V product as bf16, over a Q8 pool in two bf16 parts (16 bits).  The
+ * production shape (16, 512, 64) runs on the tensor cores and wants d_q, d_out
+ * and the pool's arrays 16-byte aligned; other shapes run a CUDA-core kernel that
+ * is right, not fast.  The outputs overlap no input.  A device-side error is
  * reported by kvl_mla_tree_check. */
 int kvl_mla_tree_attend_bf16(const KvlMlaTreePlan *plan, uint16_t *d_out, float *d_lse, const uint16_t *d_q,
                              const uint64_t *d_mask, const uint16_t *d_kv, int64_t rows, int num_heads,
@@ -266,7 +268,9 @@ int kvl_mla_tree_attend_q8(const KvlMlaTreePlan *plan, uint16_t *d_out, float *d
  * [nodes][H] fp32, d_pos [nodes].  The projections run as tensor-core GEMMs on
  * bf16-rounded activations for any number of nodes: weights, d_out, workspace
  * and pool 16-byte aligned, every width a multiple of 8, two heads at least,
- * else -1 before anything is launched.  Sequences may share cached rows (a common prefix); a
+ * else -1 before anything is launched.  The absorbed query and the latent mix
+ * are bf16 too (fp32 in a decode step): for the same token the two steps differ
+ * by 3e-3 to 4e-3 in rel-L2, as decode steps below and from 16 sequences do.  Sequences may share cached rows (a common prefix); a
  * plan where a drafted row of one is a drafted or cached row of another is
  * refused, for its append would overwrite the other's.  Workspace of
  * kvl_mla_decode_step_workspace_bytes(cfg, nodes).  Device-side errors are

@@ -62,9 +62,12 @@ class Kernel:
     """One CTA that walks items of the given numbers of tiles.  Roles are generators that yield between their steps
     and, "blocked", while they wait; `pipe` is the tensor core (in order), `loads` are copies in flight (any order)."""
 
-    def __init__(self, items, q8, steps, scales, rng):
+    def __init__(self, items, q8, steps, scales, rng, early_rope=False):
         self.items, self.q8, self.steps, self.scales, self.rng = items, q8, steps, scales, rng
-        self.full = [[Bar(1) for _ in range(steps)], [Bar(2) for _ in range(steps)]]  # unit 1: latents and rope
+        self.early_rope = early_rope  # a mistake: the rope is loaded when the scores before are done
+        self.rope_in = 0 if q8 else 1  # bf16: unit 1's barrier counts the rope too; Q8: that has its own
+        self.full = [[Bar(1) for _ in range(steps)], [Bar(1 + self.rope_in) for _ in range(steps)]]
+        self.r_full = [Bar(1), Bar(1)]
         self.done = [[Bar(1) for _ in range(steps)] for _ in range(2)]
         self.s_full, self.s_empty = [Bar(1), Bar(1)], [Bar(1), Bar(1)]
         self.q_done, self.qr_full, self.p_full, self.o_empty = Bar(1), Bar(1), Bar(1), Bar(1)
@@ -95,10 +98,11 @@ class Kernel:
 
     def producer(self):
         j = g = 0
+        step = {}  # of each tile
         for tiles in self.items:
             for h in range(2):
                 yield from self.free(j, h)
-                self.loads.append(lambda j=j, h=h: self.fill(j, h, 1 + h))
+                self.loads.append(lambda j=j, h=h: self.fill(j, h, 1 + h * self.rope_in))
                 yield
             j += 1
             for _ in range(tiles):
@@ -106,12 +110,15 @@ class Kernel:
                     yield from self.free(j, h)
                     self.loads.append(lambda j=j, h=h: self.fill(j, h, 1))
                     yield
-                if g >= 2:
+                if g >= 2 and self.q8 and not self.early_rope:  # the place of the second weights of tile g - 2
+                    yield from self.wait_done(step[g - 2], 1)
+                elif g >= 2:
                     yield from self.wait(self.s_full[g & 1], (g >> 1) - 1)
+                step[g] = j
 
                 def rope(j=j, g=g):
                     self.rope[g & 1] = g
-                    self.full[1][j % self.steps].arrive()
+                    (self.r_full[g & 1] if self.q8 else self.full[1][j % self.steps]).arrive()
 
                 self.loads.append(rope)
                 j, g = j + 1, g + 1
@@ -156,6 +163,8 @@ class Kernel:
                 if t == 0:
                     yield from self.wait(self.qr_full, n)
                 yield from self.wait_full(j, 1)
+                if self.q8:
+                    yield from self.wait(self.r_full[g & 1], g >> 1)
 
                 def score(j=j, g=g, n=n, last=t + 1 == tiles):
                     expect(self.holds(j), "scores of another step's keys")
@@ -184,6 +193,7 @@ class Kernel:
                 def product(h, j=j, g=g, n=n):
                     expect(self.ring[(2 * j + h) % UNITS] == j, "P.V with another step's rows")
                     expect(self.p == g, "P.V with another tile's weights")
+                    expect(not self.q8 or self.rope[g & 1] == ("second weights", g), "P.V with other second weights")
                     expect(self.stored >= n - 1, "P.V into an output that is not read yet")
                     self.o = g
                     self.done[h][j % self.steps].arrive()
@@ -223,6 +233,9 @@ class Kernel:
                 if g:
                     yield from self.wait_done(j - (1 if t else 2), 1)
                 self.p = g
+                if self.q8:
+                    expect(self.rope[g & 1] == g, "the rope's place holds another tile's")
+                    self.rope[g & 1] = ("second weights", g)
                 self.p_full.arrive()
                 j, g = j + 1, g + 1
                 yield
@@ -260,7 +273,7 @@ class Kernel:
                 blocked = set()
 
 
-def runs(q8, steps, scales, n, seed):
+def runs(q8, steps, scales, n, seed, **mistake):
     """How many of n random batches fail."""
     rng = random.Random(seed)
     bad = 0
@@ -268,7 +281,7 @@ def runs(q8, steps, scales, n, seed):
         items = [rng.choice([1, 2, 2, 3, 4, 5]) if rng.random() < 0.8 else rng.randint(1, 9)
                  for _ in range(rng.randint(1, 10))]
         try:
-            Kernel(items, q8, steps, scales, rng).run()
+            Kernel(items, q8, steps, scales, rng, **mistake).run()
         except (Stuck, Wrong):
             bad += 1
     return bad
@@ -292,3 +305,7 @@ def test_five_barriers_are_too_few_for_q8():
 
 def test_three_sets_of_row_scales_are_too_few():
     assert runs(True, STEPS, 3, 100, 4) > 0
+
+
+def test_the_rope_has_to_wait_for_the_second_weights():
+    assert runs(True, STEPS, SCALES, 50, 5, early_rope=True) > 0
