@@ -1819,7 +1819,7 @@ static int step_attend(const KvlMlaAttendPlan *plan, const StepPool &pool, const
 // (fp32 queries and outputs), or the nodes of drafted trees (bf16 ones: the tree
 // attend's products take no other type, and an fp32 query would only be rounded
 // there).  For one token behind 4096 rows the output of a tree step differs from
-// a decode step's by 3.3e-3 to 3.7e-3 in rel-L2, bf16 and Q8, as a decode step of
+// a decode step's by 2.9e-3 to 3.7e-3 in rel-L2, bf16 and Q8, as a decode step of
 // 16 sequences, whose activations are rounded too, does from 16 steps of one
 // (3.0e-3 to 3.8e-3).
 struct StepAttend {

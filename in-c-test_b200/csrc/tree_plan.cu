@@ -10,7 +10,7 @@
 
 namespace kvl {
 
-// In tiles (bf16 about 1.2 us, Q8 about 1.7): what an item costs beside its tiles
+// In tiles (bf16 about 1.2 us, Q8 about 2.1): what an item costs beside its tiles
 // (query, first tile, epilogue), what the merge launch costs, and a partial's 131
 // KB written and read.  Estimates from the traces of bf16 runs, used for Q8 too: a
 // plan does not know the pool that it will read.

@@ -270,11 +270,11 @@ int kvl_mla_tree_attend_q8(const KvlMlaTreePlan *plan, uint16_t *d_out, float *d
  * and pool 16-byte aligned, every width a multiple of 8, two heads at least,
  * else -1 before anything is launched.  The absorbed query and the latent mix
  * are bf16 too (fp32 in a decode step): for the same token the two steps differ
- * by 3e-3 to 4e-3 in rel-L2, as decode steps below and from 16 sequences do.  Sequences may share cached rows (a common prefix); a
- * plan where a drafted row of one is a drafted or cached row of another is
- * refused, for its append would overwrite the other's.  Workspace of
- * kvl_mla_decode_step_workspace_bytes(cfg, nodes).  Device-side errors are
- * reported by kvl_mla_tree_check. */
+ * by 3e-3 to 4e-3 in rel-L2, as decode steps of 16 sequences and of one do.
+ * Sequences may share cached rows (a common prefix); a plan where a drafted row
+ * of one is a drafted or cached row of another is refused, for its append would
+ * overwrite the other's.  Workspace of kvl_mla_decode_step_workspace_bytes(cfg,
+ * nodes).  Device-side errors are reported by kvl_mla_tree_check. */
 int kvl_mla_tree_step_bf16(const KvlMlaConfig *cfg, const KvlMlaDeviceWeights *w, const KvlMlaTreePlan *plan,
                            float *d_out, const float *d_x, const uint64_t *d_mask, const int *d_pos, uint16_t *d_kv,
                            int64_t rows, void *d_workspace, void *stream);
