@@ -128,7 +128,8 @@ constexpr uint32_t kUnit = 4 * kBox;        // half a tile's latents: 64 rows x 
 // scores and P.V of a tile in turn, a tile took 3420 cycles, of which the tensor
 // core worked about 1750).
 constexpr int kUnits = 6;
-constexpr uint32_t OFF_R = kUnits * kUnit;  // ropes of two tiles, until their scores are done; Q8: then the weights' second part
+constexpr uint32_t OFF_R = kUnits * kUnit;  // ropes of two tiles, until their scores are done;
+                                            // Q8: then the second part of their weights
 constexpr uint32_t OFF_P = OFF_R + 2 * kBox;
 constexpr uint32_t OFF_QR = OFF_P + kBox;   // the query's rope box
 constexpr uint32_t OFF_BAR = OFF_QR + kBox;

@@ -47,7 +47,8 @@ int set_tree_sequences(TreeHostPlan &hp, int batch, const int *cached_len, const
   hp = TreeHostPlan();
   hp.batch = batch;
   for (int b = 0; b < batch; ++b) {
-    if (cached_len[b] < 0 || nodes[b] < 0 || nodes[b] > kTreeMaxNodes || row0[b] < 0 || row0[b] >= (1LL << 31)) return -1;
+    if (cached_len[b] < 0 || nodes[b] < 0 || nodes[b] > kTreeMaxNodes || row0[b] < 0 || row0[b] >= (1LL << 31))
+      return -1;
     const long long end = (long long)row0[b] + cached_len[b] + nodes[b];
     if (end >= (1LL << 31)) return -1;
     hp.rows_needed = std::max(hp.rows_needed, end);
