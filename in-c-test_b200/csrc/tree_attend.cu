@@ -839,20 +839,21 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
                      (static_cast<size_t>(max(im.slot, 0)) * 64 + 32 * kh) * 128 + 32 * sub + lane;
         uint16_t *od = p.out + (static_cast<size_t>(im.node0) * kHeads + orow) * kLatent + odim;
         uint8_t *stage = smem + (odim >> 6) * kBox + (orow >> 3) * 1024 + (orow & 7) * 128;
-#pragma unroll
-        for (int c = 0; c < 128; c += 16) {
-          float o[16];
-          tmem_ld16(ocol + c, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] *= inv;
-          // A cleared row that the node sees scored -inf, with weight 0 (or its
-          // weight was NaN, and so is all of o): 0 times its elements is NaN where
-          // they are not finite, whatever other nodes of the group see.
-          if (!Q8 && cleared)
-            for (int z = 0; z < 2; ++z) {
+        // Rare, and apart from the loop below.  A cleared row that the node sees scored
+        // -inf, with weight 0 (or its weight was NaN, and so is all of o): 0 times its
+        // elements is NaN where they are not finite, whatever other nodes of the group
+        // see.  A row whose scores are all -inf gives 0, though O may hold 0 * inf; a
+        // partial keeps that, for others may have seen more.
+        const bool none = oreal && lo == 0.f && im.slot < 0;
+        if ((!Q8 && cleared) || __any_sync(0xffffffffu, none)) {
+          const int last = im.tile1 - 1;
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 16) {
+            float o[16];
+            tmem_ld16(ocol + c, o);
+            tmem_wait_ld();
+            for (int z = 0; z < 2 && !Q8; ++z) {
               if (!(cleared >> z & 1)) continue;
-              const int last = im.tile1 - 1;
               const uint16_t *v0 = p.kv + (im.row0 + kTreeKeys * (last - ((last ^ z) & 1))) * kRow + odim + c;
               for (int half = 0; half < 2; ++half)
                 for (uint32_t w = B->cleared[z][orow >> 4][half]; w; w &= w - 1) {
@@ -861,10 +862,21 @@ __global__ void __launch_bounds__(threads<Q8>(), 1) tree_attend_kernel(const __g
                   for (int i = 0; i < 16; ++i) o[i] = fmaf(0.f, __bfloat162float(__ushort_as_bfloat16(v[i])), o[i]);
                 }
             }
-          if (lo == 0.f && im.slot < 0) {  // all scores -inf, and O may hold 0 * inf
+            if (none)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = 0.f;
+              for (int i = 0; i < 16; ++i) o[i] = 0.f;
+            __syncwarp();
+            tmem_st16(ocol + c, o);
+            tmem_wait_st();
           }
+        }
+#pragma unroll
+        for (int c = 0; c < 128; c += 16) {
+          float o[16];
+          tmem_ld16(ocol + c, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] *= inv;
           if (staged) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
